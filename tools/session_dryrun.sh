@@ -14,6 +14,12 @@ T=$(mktemp -d); LOG=$T/commands.log; : > "$LOG"
 mkdir "$T/repo"
 tar c --exclude=.git --exclude=gpurun_out --exclude=tools/wavesim/_gen --exclude='*.o' --exclude=__pycache__ . | tar x -C "$T/repo"
 cd "$T/repo"
+# the variant libraries are built on demand (tools/build_variants.sh) and a fresh clone has none: every python here is a fake that
+# loads nothing, so an empty file stands in for each one that is missing and the parts that need them are dry-run everywhere
+mkdir -p cacophony_amd/_variants
+for v in skew skew_lin classic attn_lean attn_lean_k2 wb hints r2 libm_erf r2addr; do
+  [ -e cacophony_amd/_variants/libcaco_hip_$v.so ] || : > cacophony_amd/_variants/libcaco_hip_$v.so
+done
 source tools/session_fakes.sh "$T" "$LOG"
 export OUT=$T/out          # gpu_session.sh's own record directory
 FAIL=0
