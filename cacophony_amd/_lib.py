@@ -64,6 +64,11 @@ _SIGNATURES = {
     "caco_similarity_ld": (C.c_int, [_vp, _i32, _i32, _vp, _i32, _i32, _i32, _f32, _vp, _i32, _vp]),
     "caco_l2_normalize": (C.c_int, [_vp, _i32, _i32, _vp, _vp]),
     "caco_topk": (C.c_int, [_vp, _i32, _i32, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "caco_linear_loss_workspace": (_i64, [_i64, _i32, _i32, _i32, _i64, _i32]),
+    "caco_linear_ce": (C.c_int, [_i32, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _i32, _i32] + [_vp] * 5 +
+                       [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp]),
+    "caco_linear_distill": (C.c_int, [_i32, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i32, _i32, _f32, _i64, _i32, _i32, _i32] +
+                            [_vp] * 5 + [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp]),
     "caco_token_group_mean": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _vp, _vp]),
     "caco_mae_forward": (C.c_int, [_vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp]),
     "caco_workspace_bytes": (_i64, [_vp]),

@@ -1246,6 +1246,45 @@ int caco_topk(const float* sim, int32_t rows, int32_t cols, int64_t row_stride, 
   return CACO_OK;
 }
 
+int64_t caco_linear_loss_workspace(int64_t rows, int32_t vocab, int32_t dim, int32_t topk, int64_t piece_bytes, int32_t what) {
+  return linear_loss_workspace(rows, vocab, dim, topk, piece_bytes, what);
+}
+
+int caco_linear_ce(int32_t what, const void* hidden, int64_t ld_h, const void* weight, int64_t ld_w, const float* bias,
+                   const int64_t* labels, int64_t ignore_index, int64_t rows, int32_t vocab, int32_t dim, int32_t reduction,
+                   const float* row_weight, const float* grad_scale, float* row_loss, float* lse, float* loss, void* d_hidden,
+                   int64_t ld_dh, void* d_weight, int64_t ld_dw, float* d_bias, void* ws, int64_t ws_bytes, void* stream) {
+  LinearLoss c{};
+  c.what = what; c.hidden = (const bf16_t*)hidden; c.ld_h = ld_h; c.weight = (const bf16_t*)weight; c.ld_w = ld_w; c.bias = bias;
+  c.labels = labels; c.ignore_index = ignore_index;
+  c.rows = rows; c.vocab = vocab; c.dim = dim; c.reduction = reduction; c.row_weight = row_weight; c.grad_scale = grad_scale;
+  c.row_loss = row_loss; c.lse = lse; c.loss = loss;
+  c.d_hidden = (bf16_t*)d_hidden; c.ld_dh = ld_dh; c.d_weight = (bf16_t*)d_weight; c.ld_dw = ld_dw; c.d_bias = d_bias;
+  c.ws = ws; c.ws_bytes = ws_bytes;
+  hipStream_t st = (hipStream_t)stream;
+  CACO_STAGE("loss.linear_ce", linear_loss(c, st));
+  return CACO_OK;
+}
+
+int caco_linear_distill(int32_t what, const void* hidden, int64_t ld_h, const void* weight, int64_t ld_w, const float* bias,
+                        const float* teacher, int64_t ld_t, const void* teacher_idx, int64_t ld_i, int32_t idx_bytes, int32_t topk,
+                        float temperature, int64_t rows, int32_t vocab, int32_t dim, int32_t reduction, const float* row_weight,
+                        const float* grad_scale, float* row_loss, float* lse, float* loss, void* d_hidden, int64_t ld_dh,
+                        void* d_weight, int64_t ld_dw, float* d_bias, void* ws, int64_t ws_bytes, void* stream) {
+  CACO_REQUIRE(idx_bytes == 4 || idx_bytes == 8, "caco_linear_distill: idx_bytes must be 4 or 8");
+  CACO_REQUIRE(topk >= 1, "caco_linear_distill: topk must be 1 .. 128, got %d", topk);
+  LinearLoss c{};
+  c.what = what; c.hidden = (const bf16_t*)hidden; c.ld_h = ld_h; c.weight = (const bf16_t*)weight; c.ld_w = ld_w; c.bias = bias;
+  c.teacher = teacher; c.ld_t = ld_t; c.teacher_idx = teacher_idx; c.ld_i = ld_i; c.idx64 = idx_bytes == 8; c.topk = topk; c.temperature = temperature;
+  c.rows = rows; c.vocab = vocab; c.dim = dim; c.reduction = reduction; c.row_weight = row_weight; c.grad_scale = grad_scale;
+  c.row_loss = row_loss; c.lse = lse; c.loss = loss;
+  c.d_hidden = (bf16_t*)d_hidden; c.ld_dh = ld_dh; c.d_weight = (bf16_t*)d_weight; c.ld_dw = ld_dw; c.d_bias = d_bias;
+  c.ws = ws; c.ws_bytes = ws_bytes;
+  hipStream_t st = (hipStream_t)stream;
+  CACO_STAGE("loss.linear_distill", linear_loss(c, st));
+  return CACO_OK;
+}
+
 int caco_token_group_mean(const float* hidden, int32_t batch, int32_t seq, int32_t dim, int32_t group, float* out, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   CACO_STAGE("hear.token_group_mean", token_group_mean(hidden, batch, seq, dim, group, out, st));

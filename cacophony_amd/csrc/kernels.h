@@ -131,6 +131,25 @@ int token_group_mean(const float* x, int batch, int seq, int hidden, int group, 
 int topk_rows(const float* sim, int rows, int cols, int64_t row_stride, int64_t col_stride, int k, int* idx, float* val,
               hipStream_t st);
 
+// linear_loss.hip: losses of a linear vocabulary head without its logits (include/caco_hip.h: caco_linear_ce, caco_linear_distill)
+struct LinearLoss {
+  int what;                          // CACO_LOSS_FORWARD | CACO_LOSS_BACKWARD
+  const bf16_t* hidden; int64_t ld_h;
+  const bf16_t* weight; int64_t ld_w;
+  const float* bias;
+  const int64_t* labels; int64_t ignore_index;                                   // cross entropy (topk = 0)
+  const float* teacher; int64_t ld_t; const void* teacher_idx; int64_t ld_i; int idx64; int topk; float temperature;      // distillation
+  int64_t rows; int vocab, dim, reduction;
+  const float* row_weight; const float* grad_scale;
+  float *row_loss, *lse, *loss;
+  bf16_t* d_hidden; int64_t ld_dh;
+  bf16_t* d_weight; int64_t ld_dw;
+  float* d_bias;
+  void* ws; int64_t ws_bytes;
+};
+int64_t linear_loss_workspace(int64_t rows, int32_t vocab, int32_t dim, int32_t topk, int64_t piece_bytes, int32_t what);
+int linear_loss(const LinearLoss& c, hipStream_t st);
+
 // mel.hip
 // lengths: int64 [batch] valid samples per clip (device), or null = every clip is n_samples long
 int mel_frontend(const float* wav, int batch, int64_t n_samples, int max_patches, float scale, float bias,

@@ -190,6 +190,49 @@ int caco_decode_begin(caco_model* m, const float* audio_hidden_dev, const float*
 int caco_decode_step(caco_decode_state* s, const int64_t* token_ids_dev, float* logits_dev, void* stream);
 void caco_decode_end(caco_decode_state* s);
 
+/* ---- losses of a linear vocabulary head, logits never kept ---------------------------------------------------------------------
+ * z = hidden . weight^T + bias: hidden_dev bf16 [rows, dim] (row stride ld_h), weight_dev bf16 [vocab, dim] (ld_w), bias_dev fp32
+ * [vocab] or NULL - the layout of `decoder_proj` (src/caco_torch/text_models/roberta.py:371).  The reference materialises the logits
+ * of get_decoder_logits (src/caco_torch/caco.py:212-240) for whatever it computes from them; these calls compute the loss of every
+ * row and, if asked, the gradients, in pieces of the vocabulary.  Sums, softmax statistics and gradients of the bias are fp32.
+ *
+ * caco_linear_ce: row loss = logsumexp(z) - z[label].  A row whose label is ignore_index or outside [0, vocab) does not count: its loss
+ *   is 0, its gradient is 0, and its hidden state - NaN or not - reaches nothing.
+ * caco_linear_distill: distillation from a teacher's `topk` (1 .. 128) best logits per row (caco_topk gives them): teacher_dev fp32
+ *   [rows, topk] (ld_t), teacher_idx_dev int32 or int64 (idx_bytes 4 or 8) [rows, topk] (ld_i).  q = softmax(teacher / T) over the row's
+ *   entries, row loss = T^2 * sum_k q_k (log q_k - log softmax(z / T)[i_k]).  An index outside [0, vocab) (caco_topk pads with -1) or a
+ *   logit of -inf is no entry; entries of one token add up; a row without entries does not count.
+ * `what`: CACO_LOSS_FORWARD writes row_loss_dev fp32 [rows], lse_dev fp32 [rows] (logsumexp of z, of z / T for the distillation; may be
+ *   NULL when the backward pass is not a later call) and, for a reduction other than CACO_REDUCE_NONE, loss_dev fp32 [1] (may be NULL) = sum of
+ *   row_weight * row_loss, divided for CACO_REDUCE_MEAN by the number of rows that count (NaN if none does).  CACO_LOSS_BACKWARD
+ *   writes the gradients of that scalar times *grad_scale_dev (for CACO_REDUCE_NONE: of the weighted sum): d_hidden_dev bf16
+ *   [rows, dim] (ld_dh), d_weight_dev bf16 [vocab, dim] (ld_dw), d_bias_dev fp32 [vocab]; each may be NULL, not all.  It reads lse_dev
+ *   unless the forward pass is part of the same call (CACO_LOSS_FORWARD | CACO_LOSS_BACKWARD).  No row counts: zero gradients.
+ *   row_weight_dev fp32 [rows] or NULL (= 1), grad_scale_dev fp32 [1] or NULL (= 1).
+ * Row strides are in elements, >= dim and multiples of 8, and rows start at multiples of 16 bytes; dim is a multiple of 8; rows <= 2^24
+ *   (0 is allowed), vocab <= 2^24, dim <= 65536.
+ * ws_dev: scratch of the caller's, 16-byte aligned, its contents are not kept; one call at a time may use it.  caco_linear_loss_workspace
+ *   gives its size (topk 0 = cross entropy; < 0: CACO_ERR_INVALID); with the backward pass it includes the gradient of the logits
+ *   for one piece of the vocabulary in bf16, of about piece_bytes (at least 256 columns).  A smaller workspace makes more pieces.
+ * Capturable into a graph: no synchronisation, no allocation, no memset; equal calls give equal bits. */
+#define CACO_LOSS_FORWARD 1
+#define CACO_LOSS_BACKWARD 2
+#define CACO_REDUCE_NONE 0
+#define CACO_REDUCE_MEAN 1
+#define CACO_REDUCE_SUM 2
+int64_t caco_linear_loss_workspace(int64_t rows, int32_t vocab, int32_t dim, int32_t topk, int64_t piece_bytes, int32_t what);
+int caco_linear_ce(int32_t what, const void* hidden_dev, int64_t ld_h, const void* weight_dev, int64_t ld_w, const float* bias_dev,
+                   const int64_t* labels_dev, int64_t ignore_index, int64_t rows, int32_t vocab, int32_t dim, int32_t reduction,
+                   const float* row_weight_dev, const float* grad_scale_dev, float* row_loss_dev, float* lse_dev, float* loss_dev,
+                   void* d_hidden_dev, int64_t ld_dh, void* d_weight_dev, int64_t ld_dw, float* d_bias_dev, void* ws_dev,
+                   int64_t ws_bytes, void* stream);
+int caco_linear_distill(int32_t what, const void* hidden_dev, int64_t ld_h, const void* weight_dev, int64_t ld_w, const float* bias_dev,
+                        const float* teacher_dev, int64_t ld_t, const void* teacher_idx_dev, int64_t ld_i, int32_t idx_bytes,
+                        int32_t topk, float temperature, int64_t rows, int32_t vocab, int32_t dim, int32_t reduction,
+                        const float* row_weight_dev, const float* grad_scale_dev, float* row_loss_dev, float* lse_dev, float* loss_dev,
+                        void* d_hidden_dev, int64_t ld_dh, void* d_weight_dev, int64_t ld_dw, float* d_bias_dev, void* ws_dev,
+                        int64_t ws_bytes, void* stream);
+
 /* ---- introspection / measurement ---------------------------------------------------------------- */
 int64_t caco_workspace_bytes(const caco_model* m);
 /* Tuning knob (process-global): bf16 GEMM kernel choice.  256 (default) = per shape: the persistent 256x256 eight-wave
