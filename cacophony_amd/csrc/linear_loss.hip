@@ -11,17 +11,19 @@
 //   compact      row numbers of the rows that count, in order; how many
 //   gather       those rows of `hidden`, next to one another, padded with zero rows and columns: a row that does not count takes no
 //                part in any product, so whatever its hidden state holds (NaN, infinities) reaches nothing
-//   lse          logits tile by tile, every lane keeping a running maximum and sum of its own columns; a workgroup walks a slice of
-//                the vocabulary for one block of rows, slices are joined by `finish`
-//   finish       row losses in the caller's order, lse
+//   lse          logits tile by tile; a workgroup stays with a block of rows for many tiles of the vocabulary, every lane keeps a sum of
+//                exp2 over its own columns against a reference that only moves when a sum would leave the range (see lse_body)
+//   finish       row losses in the caller's order, lse: a wave joins the workgroups that shared the row
 //   reduce       their sum or mean in a fixed order
 // and for the gradients, one piece of the vocabulary after the other (as many columns as the workspace holds):
 //   dlogits      the same products again, then g (p - q) rounded to bf16: the operand type of the two products that follow.  The
 //                rounding is 2^-9 of each entry, independent from entry to entry, and the targets are subtracted before it.
 //                Column sums for d bias are taken from the unrounded values.
-//   dhidden      split over the vocabulary into fp32 slabs that later pieces add to; `dh_join` adds the slabs in order
-//   dweight      the piece's rows of d weight, complete
-// Nothing is accumulated with atomics: equal calls give equal bits.
+//   targets2     (distillation) the entries of the teacher's tokens, from the logits that the loss was taken from
+//   grads        d weight's tiles (sums over the tokens, complete) and d hidden (sums over the vocabulary, cut into one run per
+//                workgroup that makes up for the uneven number of d weight's tiles; partial sums are kept in fp32)
+//   dh_join      adds the partial sums in order, one rounding
+// Nothing is accumulated in an order that can change: equal calls give equal bits.
 #define CACO_WAVE_SYNC_FENCE
 #include "common.h"
 #include "kernels.h"
@@ -32,7 +34,7 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int MAX_WG = 512;          // most workgroups of a persistent launch (two per CU)
-constexpr int DH_UNITS = 512;        // (row block, column block, slab) units that fill the chip in `dhidden`
+constexpr int MAX_CU = 256;
 
 typedef VgTile<8, 4, 2, 4> Big;      // 256 x 256, one workgroup per CU
 typedef VgTile<4, 2, 1, 4> Small;    // 64 x 128, two per CU: 64 tokens or fewer, where a call reads the weights and does little else
@@ -61,14 +63,16 @@ struct LossArgs {
   int *tgt_idx0; float *tgt_q0;      // targets in the caller's order [rows, kp] (distillation)
   int *tgt_idx; float *tgt_q;        // targets of the compact rows [npad, kp]
   bf16_t* hc;                        // [npad, hp]
-  float2* part;                      // (max, sum) of log2-logits, [slice][row block rows]
-  float* zt;                         // cross entropy: the label's log2-logit; distillation: sum_k q_k (log q_k - z_k / T)
+  float2* part;                      // (max, sum) of log2-logits, [group of row blocks][workgroup][rows of a block]
+  float* zt;                         // cross entropy: the label's log2-logit; distillation: sum_k q_k (z_k / T - log q_k), log2 units
+  float* tgt_z;                      // distillation: the entries' log2-logits [npad, kp]
   float *lse2, *g;                   // compact: lse in log2 units, gradient scale of the row
+  unsigned* gmax;                    // bits of the largest |g|
+  unsigned long long* db64;          // distillation: sum of the targets' weights per word, fixed point in units of 2^(e - 38), |g| < 2^e
   bf16_t* dl;                        // [npad, piece]
-  float* slab;                       // [slabs][row blocks * BM, hs]
+  float* slab;                       // d hidden's partial sums [output tile + workgroup][256][256]
   float* dbp;                        // [row halves, piece]
   int piece, v0;                     // columns of the piece, its first column
-  int hs;                            // columns of a slab row
 };
 
 // ------------------------------------------------------------------------------------------------------------------------------------
@@ -163,7 +167,10 @@ __global__ __launch_bounds__(1024) void compact_kernel(LossArgs a) {
     a.inv[r] = c ? at : -1;
     if (c) a.rowmap[at++] = (int)r;
   }
-  if (tid == 1023) *a.count = at;
+  if (tid == 1023) {
+    *a.count = at;
+    *a.gmax = 0;
+  }
 }
 
 // compact row <- its hidden state, targets, gradient scale.  One wave per row; rows up to the next multiple of 256 are zero rows.
@@ -171,6 +178,8 @@ __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, i
   const int lane = threadIdx.x & 63;
   const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int n = *a.count;
+  if (backward && a.db && a.topk)
+    for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < a.vocab; v += (int64_t)gridDim.x * 256) a.db64[v] = 0;
   if (c >= ((int64_t)n + 255) / 256 * 256) return;
   const bool real = c < n;
   const int64_t row = real ? a.rowmap[c] : 0;
@@ -193,6 +202,7 @@ __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, i
     if (real && a.grad_scale) g *= *a.grad_scale;
     if (real && a.reduction == CACO_REDUCE_MEAN) g /= (float)n;
     a.g[c] = g;
+    atomicMax(a.gmax, __float_as_uint(fabsf(g)));      // a maximum does not depend on the order
     if (from_lse) a.lse2[c] = real ? a.lse[row] * LOG2E : 0.f;
   }
 }
@@ -222,7 +232,9 @@ __global__ __launch_bounds__(256) void target_logits_kernel(LossArgs a) {
     for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
     if (q != 0.f && l16 == 0) {      // 0 log 0 = 0: an entry of weight 0 (or none) adds nothing, whatever its logit is
       if (a.bias) z += a.bias[idx];
-      sum += q * (log2f(q) - z * a.inv_t * LOG2E);
+      z *= a.inv_t * LOG2E;
+      sum += q * (log2f(q) - z);
+      a.tgt_z[c * a.kp + k] = z;
     }
   }
   sum = wave_sum(sum);
@@ -230,120 +242,211 @@ __global__ __launch_bounds__(256) void target_logits_kernel(LossArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
-// logits -> running maximum and sum
+// logits -> running sums of exponentials
 // ------------------------------------------------------------------------------------------------------------------------------------
-// Units (row block, slice of the vocabulary's tiles).  Consecutive units go to one XCD, slices of a row block next to one another:
-// an XCD's L2 holds the few row blocks its workgroups share while their slices of the weights stream through it.
-struct LseUnits {
-  int rb, tiles, slices, units;
-  __device__ __forceinline__ LseUnits(int n, int vocab, int bm, int bn, int wgs) {
+// The order of the (row block, vocabulary tile) pairs.  Row blocks in groups of 8, then 4, 2, 1; inside a group the vocabulary's tiles, row blocks
+// fastest.  An XCD takes a run of consecutive pairs, its workgroups one after the other: 8 panels of hidden states stay in its L2 and a
+// panel of weights is used 8 times while it is there.  The width of a group divides the number of an XCD's workgroups, so a workgroup
+// keeps its row block for a whole group.
+struct Order {
+  int rb, tiles, units;
+  int slots, cnt, base;              // of this XCD: workgroups, pairs, first pair
+  __device__ __forceinline__ Order(int n, int vocab, int bm, int bn, int wgs, int xcd) {
     rb = (n + bm - 1) / bm;
     tiles = (vocab + bn - 1) / bn;
-    slices = rb > 0 ? max(1, min(tiles, wgs / rb)) : 1;
-    units = rb * slices;
+    units = rb * tiles;
+    slots = wgs >> 3;
+    cnt = (units >> 3) + (xcd < (units & 7) ? 1 : 0);
+    base = xcd * (units >> 3) + min(xcd, units & 7);
+  }
+};
+struct Walk {
+  int t, end;                        // pair, the run's end
+  int rb, vt;                        // what it is
+  int group, lw, gend;               // number of the group, log2 of its width, the pair behind it
+  __device__ __forceinline__ void set(const Order& o) {
+    const int full = o.rb >> 3;
+    int g0 = 0, gs = 0;
+    lw = 3;
+    if (t < full * 8 * o.tiles) {
+      group = t / (8 * o.tiles);
+      g0 = group * 8;
+      gs = g0 * o.tiles;
+    } else {
+      group = full - 1;
+      g0 = full * 8;
+      for (int l = 2; l >= 0; --l)
+        if ((o.rb >> l) & 1) {
+          ++group;
+          gs = g0 * o.tiles;
+          lw = l;
+          if (t < gs + (o.tiles << l)) break;
+          g0 += 1 << l;
+        }
+    }
+    gend = gs + (o.tiles << lw);
+    rb = g0 + ((t - gs) & ((1 << lw) - 1));
+    vt = (t - gs) >> lw;
+  }
+  __device__ __forceinline__ Walk(const Order& o, int slot) : t(o.base + slot), end(o.base + o.cnt) { if (t < end) set(o); }
+  __device__ __forceinline__ int left(const Order& o) const { return t < end ? (end - t + o.slots - 1) / o.slots : 0; }
+  __device__ __forceinline__ bool last_of_group(const Order& o) const { return t + o.slots >= min(gend, end); }
+  __device__ __forceinline__ void next(const Order& o) {
+    t += o.slots;
+    if (t < gend) vt += o.slots >> lw;
+    else if (t < end) set(o);
+  }
+};
+// groups of at most `rb` row blocks
+__host__ __device__ inline int64_t most_groups(int64_t rb) { return rb / 8 + 3; }
+
+// The words of an output tile: bias of its columns, labels (and for d logits lse and g) of its rows.
+template <typename C>
+struct Words {
+  static constexpr int BIAS = 0, Y = C::BN * 4, LSE = Y + C::BM * 4, G = LSE + C::BM * 4;
+  static __device__ __forceinline__ void bring(const LossArgs& a, int n0, int64_t m0, bool grad, char* lds) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int pc = wave; pc < (C::BN + (grad ? 3 : 1) * C::BM) / 64; pc += C::WAVES) {
+      if (pc < C::BN / 64) {
+        if (a.bias) vg_words(a.bias + min(n0 + pc * 64, a.vocab), a.vocab - n0 - pc * 64, lds + BIAS + pc * 256, lane);
+        continue;
+      }
+      const int r = pc - C::BN / 64, which = r / (C::BM / 64), m = r % (C::BM / 64) * 64;
+      if (which == 0 && !a.topk) vg_words(a.tgt_idx + m0 + m, 64, lds + Y + m * 4, lane);
+      if (which == 1) vg_words(a.lse2 + m0 + m, 64, lds + LSE + m * 4, lane);
+      if (which == 2) vg_words(a.g + m0 + m, 64, lds + G + m * 4, lane);
+    }
+  }
+  // sums begin with the bias; a column past the vocabulary with -inf, its logit and nothing else comes of it
+  static __device__ __forceinline__ void start(const LossArgs& a, int n0, int wn, int lq, const char* lds, f32x4 (&acc)[C::MI][C::NI]) {
+    const bool edge = n0 + C::BN > a.vocab;
+#pragma unroll
+    for (int j = 0; j < C::NI; ++j) {
+      const int c = wn * 16 * C::NI + j * 16 + lq * 4;
+      f32x4 b = {0.f, 0.f, 0.f, 0.f};
+      if (a.bias) b = *reinterpret_cast<const f32x4*>(lds + BIAS + c * 4);
+      if (edge)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n0 + c + e >= a.vocab) b[e] = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < C::MI; ++i) acc[i][j] = b;
+    }
   }
 };
 
+// Per element one multiply-add, one v_exp_f32 and one addition.  The reference of a lane's row is the maximum over the row's first tile of
+// this wave (four lanes share it) and stays there while the sums stay below 2^100; when one does not (or is NaN) the whole wave goes
+// over the tile again with its maxima.  Logits far below the reference add what they should: nothing.
 template <typename C>
 __device__ __forceinline__ void lse_body(const LossArgs& a, char* smem) {
   const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
-  const int n = *a.count;
-  const LseUnits U(n, a.vocab, C::BM, C::BN, gridDim.x);
-  const int wg = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  const Order O(*a.count, a.vocab, C::BM, C::BN, gridDim.x, blockIdx.x & 7);
+  const int wg = (blockIdx.x & 7) * O.slots + (blockIdx.x >> 3);
+  Walk L(O, blockIdx.x >> 3), A = L, M = L;      // operands, words, sums
+  const int tiles = M.left(O);
+  if (tiles == 0) return;
   const float cs = a.inv_t * LOG2E;
-  const bool label = a.labels != nullptr;
-  for (int u = wg; u < U.units; u += gridDim.x) {
-    const int rb = u / U.slices, sl = u % U.slices;
-    const int t0 = (int)((int64_t)sl * U.tiles / U.slices), t1 = (int)((int64_t)(sl + 1) * U.tiles / U.slices);
-    const int64_t m0 = (int64_t)rb * C::BM;
-    float mx[C::MI], sm[C::MI];
-    int y[C::MI];
+  const bool label = !a.topk;
+  float nref[C::MI], sm[C::MI];      // minus the reference, the sum
 #pragma unroll
-    for (int i = 0; i < C::MI; ++i) {
-      mx[i] = -3.0e38f;            // finite: exp2(-inf - mx) = 0 for logits of -inf
-      sm[i] = 0.f;
-      y[i] = label ? a.tgt_idx[m0 + (wm * C::MI + i) * 16 + l16] : -1;
-    }
-    vg_run<C, false, false>(
-        t1 - t0, smem,
-        [&](int i, VgOperand& X, VgOperand& W, int& k0, int& k1) {
-          const int n0 = (t0 + i) * C::BN;
-          X = VgOperand{a.hc + m0 * a.hp, a.hp, C::BM, a.hp};
-          W = VgOperand{a.weight + (int64_t)n0 * a.ld_w, a.ld_w, a.vocab - n0, a.dim};
-          k0 = 0;
-          k1 = a.hp / VG_K;
-        },
-        [&](int i, f32x4 (&acc)[C::MI][C::NI]) {
-          const int n0 = (t0 + i) * C::BN + wn * 16 * C::NI + lq * 4;      // this lane's columns: n0 + j * 16 + e
-          float b2[C::NI][4];
+  for (int q = 0; q < C::MI; ++q) { nref[q] = 3.0e38f; sm[q] = 0.f; }
+  vg_run<C, false, false, true>(
+      tiles, smem,
+      [&](int, int& k0, int& k1) { k0 = 0; k1 = a.hp / VG_K; },
+      [&](int, VgOperand& X, VgOperand& W) {
+        const int n0 = L.vt * C::BN;
+        X = VgOperand{a.hc + (int64_t)L.rb * C::BM * a.hp, a.hp, C::BM, a.hp};
+        W = VgOperand{a.weight + (int64_t)n0 * a.ld_w, a.ld_w, a.vocab - n0, a.dim};
+        L.next(O);
+      },
+      [&](int, char* w) {
+        Words<C>::bring(a, A.vt * C::BN, (int64_t)A.rb * C::BM, false, w);
+        A.next(O);
+      },
+      [&](int, f32x4 (&acc)[C::MI][C::NI], char* w) { Words<C>::start(a, M.vt * C::BN, wn, lq, w, acc); },
+      [&](int, f32x4 (&acc)[C::MI][C::NI], char* w) {
+        const int rb = M.rb, tn = M.vt;
+        const int n0 = tn * C::BN + wn * 16 * C::NI + lq * 4;      // this lane's columns: n0 + j * 16 + e
+#pragma unroll
+        for (int q = 0; q < C::MI; ++q) {
+          float s[4] = {sm[q], 0.f, 0.f, 0.f};
 #pragma unroll
           for (int j = 0; j < C::NI; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int v = n0 + j * 16 + e;
-              b2[j][e] = v < a.vocab ? (a.bias ? a.bias[v] * cs : 0.f) : -INFINITY;
-            }
+            for (int e = 0; e < 4; ++e) s[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[q][j][e], cs, nref[q]));
+          s[0] = (s[0] + s[1]) + (s[2] + s[3]);
+          if (__ballot(!(s[0] < 0x1p100f))) {
+            float m = -nref[q];
+#pragma unroll
+            for (int j = 0; j < C::NI; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) m = fmaxf(m, acc[q][j][e] * cs);
+            m = fmaxf(m, __shfl_xor(m, 16, 64));
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            s[0] = sm[q] * __builtin_amdgcn_exp2f(-nref[q] - m);
+#pragma unroll
+            for (int j = 0; j < C::NI; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[0] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[q][j][e], cs, -m));
+            nref[q] = -m;
+          }
+          sm[q] = s[0];
+        }
+        if (label) {
 #pragma unroll
           for (int q = 0; q < C::MI; ++q) {
-            float z[C::NI][4];
-            float m = mx[q];
-#pragma unroll
-            for (int j = 0; j < C::NI; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                z[j][e] = b2[j][e] == -INFINITY ? -INFINITY : __builtin_fmaf(acc[q][j][e], cs, b2[j][e]);
-                m = fmaxf(m, z[j][e]);
-              }
-            float s = sm[q] * __builtin_amdgcn_exp2f(mx[q] - m);
-#pragma unroll
-            for (int j = 0; j < C::NI; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(z[j][e] - m);
-            mx[q] = m;
-            sm[q] = s;
-            const int d = y[q] - n0;                       // the label's place among this lane's columns
+            const int row = (wm * C::MI + q) * 16 + l16;
+            const int d = *reinterpret_cast<const int*>(w + Words<C>::Y + row * 4) - n0;      // the label's place among this lane's columns
             if ((unsigned)d < 16u * C::NI && (d & 12) == 0) {
               float zy = 0.f;
 #pragma unroll
               for (int j = 0; j < C::NI; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                  if (d == j * 16 + e) zy = z[j][e];
-              a.zt[m0 + (wm * C::MI + q) * 16 + l16] = zy;
+                  if (d == j * 16 + e) zy = acc[q][j][e] * cs;
+              a.zt[(int64_t)rb * C::BM + row] = zy;
             }
           }
-        });
-    // the four lanes of a row, then the waves that share it
-    float2* red = reinterpret_cast<float2*>(vg_slab<C>(smem, 0));      // [WN][BM]
-    static_assert(C::WN * C::BM * 8 <= C::WAVES * C::SLAB, "the joint of the waves fits the slabs");
+        }
+        const bool more = !M.last_of_group(O);
+        const int part = M.group * gridDim.x + wg;
+        M.next(O);
+        if (more) return;
+        // the last tile of this row block here: the four lanes of a row, then the waves that share it
+        float2* red = reinterpret_cast<float2*>(smem + C::O_SLAB);      // [WN][BM]
+        static_assert(C::WN * C::BM * 8 <= C::WAVES * C::SLAB, "the joint of the waves fits the slabs");
+        __syncthreads();
 #pragma unroll
-    for (int q = 0; q < C::MI; ++q) {
-      float m = mx[q], s = sm[q];
+        for (int q = 0; q < C::MI; ++q) {
+          float m = -nref[q], s = sm[q];
 #pragma unroll
-      for (int o = 16; o <= 32; o <<= 1) {
-        const float om = __shfl_xor(m, o, 64), os = __shfl_xor(s, o, 64);
-        const float nm = fmaxf(m, om);
-        s = s * __builtin_amdgcn_exp2f(m - nm) + os * __builtin_amdgcn_exp2f(om - nm);
-        m = nm;
-      }
-      if (lq == 0) red[wn * C::BM + (wm * C::MI + q) * 16 + l16] = make_float2(m, s);
-    }
-    __syncthreads();
-    for (int r = threadIdx.x; r < C::BM; r += C::THREADS) {
-      float m = red[r].x, s = red[r].y;
+          for (int o = 16; o <= 32; o <<= 1) {
+            const float om = __shfl_xor(m, o, 64), os = __shfl_xor(s, o, 64);
+            const float nm = fmaxf(m, om);
+            s = s * __builtin_amdgcn_exp2f(m - nm) + os * __builtin_amdgcn_exp2f(om - nm);
+            m = nm;
+          }
+          if (lq == 0) red[wn * C::BM + (wm * C::MI + q) * 16 + l16] = make_float2(m, s);
+          nref[q] = 3.0e38f;
+          sm[q] = 0.f;
+        }
+        __syncthreads();
+        for (int r = threadIdx.x; r < C::BM; r += C::THREADS) {
+          float m = red[r].x, s = red[r].y;
 #pragma unroll
-      for (int w = 1; w < C::WN; ++w) {
-        const float2 o = red[w * C::BM + r];
-        const float nm = fmaxf(m, o.x);
-        s = s * __builtin_amdgcn_exp2f(m - nm) + o.y * __builtin_amdgcn_exp2f(o.x - nm);
-        m = nm;
-      }
-      a.part[(int64_t)sl * U.rb * C::BM + m0 + r] = make_float2(m, s);
-    }
-    __syncthreads();               // the next unit's run fills the stages, its joint the slabs
-  }
+          for (int v = 1; v < C::WN; ++v) {
+            const float2 o = red[v * C::BM + r];
+            const float nm = fmaxf(m, o.x);
+            s = s * __builtin_amdgcn_exp2f(m - nm) + o.y * __builtin_amdgcn_exp2f(o.x - nm);
+            m = nm;
+          }
+          a.part[(int64_t)part * C::BM + r] = make_float2(m, s);
+        }
+      });
 }
 template <typename C>
 __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void lse_kernel(LossArgs a) {
@@ -351,7 +454,7 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
   lse_body<C>(a, smem);
 }
 
-// One wave per row of the caller: joins the slices, row loss and lse; rows that do not count get zeros.
+// One wave per row of the caller: joins the row's parts, row loss and lse; rows that do not count get zeros.
 __global__ __launch_bounds__(256) void finish_kernel(LossArgs a, int bm, int bn, int wgs) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -364,13 +467,32 @@ __global__ __launch_bounds__(256) void finish_kernel(LossArgs a, int bm, int bn,
     }
     return;
   }
-  const LseUnits U(*a.count, a.vocab, bm, bn, wgs);
+  const int rb = c / bm;
   float m = -3.0e38f, s = 0.f;
-  for (int sl = lane; sl < U.slices; sl += 64) {
-    const float2 o = a.part[(int64_t)sl * U.rb * bm + c];
-    const float nm = fmaxf(m, o.x);
-    s = s * __builtin_amdgcn_exp2f(m - nm) + o.y * __builtin_amdgcn_exp2f(o.x - nm);
-    m = nm;
+  for (int w = lane; w < wgs; w += 64) {      // the workgroups that had this row block: their first pair of its group
+    const Order O(*a.count, a.vocab, bm, bn, wgs, w / (wgs >> 3));
+    // the group of rb and its pairs
+    const int full = O.rb >> 3;
+    int group = rb >> 3, g0 = group * 8, lw = 3;
+    if (group >= full) {
+      group = full - 1;
+      g0 = full * 8;
+      for (int l = 2; l >= 0; --l)
+        if ((O.rb >> l) & 1) {
+          ++group;
+          lw = l;
+          if (rb < g0 + (1 << l)) break;
+          g0 += 1 << l;
+        }
+    }
+    const int lo = max(g0 * O.tiles, O.base), hi = min(g0 * O.tiles + (O.tiles << lw), O.base + O.cnt);
+    const int t = lo + ((O.base + w % O.slots - lo) & (O.slots - 1));
+    if (t < hi && ((t - g0 * O.tiles) & ((1 << lw) - 1)) == rb - g0) {
+      const float2 o = a.part[(int64_t)(group * wgs + w) * bm + c % bm];
+      const float nm = fmaxf(m, o.x);
+      s = s * __builtin_amdgcn_exp2f(m - nm) + o.y * __builtin_amdgcn_exp2f(o.x - nm);
+      m = nm;
+    }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -381,9 +503,9 @@ __global__ __launch_bounds__(256) void finish_kernel(LossArgs a, int bm, int bn,
   }
   if (lane == 0) {
     const float l2 = m + log2f(s);
-    if (a.lse2) a.lse2[c] = l2;
+    a.lse2[c] = l2;
     if (a.lse) a.lse[row] = l2 * LN2;
-    if (a.row_loss) a.row_loss[row] = (l2 - a.zt[c]) * LN2 * a.temperature * a.temperature;
+    a.row_loss[row] = (l2 - a.zt[c]) * LN2 * a.temperature * a.temperature;
   }
 }
 
@@ -408,113 +530,83 @@ __global__ __launch_bounds__(1024) void reduce_kernel(LossArgs a) {
 // ------------------------------------------------------------------------------------------------------------------------------------
 // gradients
 // ------------------------------------------------------------------------------------------------------------------------------------
-// Tile order of a piece: an XCD takes a run of consecutive tiles; blocks of 8 row blocks, inside them the vocabulary's tiles, row blocks
-// fastest: 8 panels of hidden states stay in the XCD's L2 and a panel of weights is used 8 times while it is there.
-struct Order2 {
-  int a, b, units, q, r;
-  __device__ __forceinline__ Order2(int a_, int b_) : a(a_), b(b_), units(a_ * b_), q(units >> 3), r(units & 7) {}
-  __device__ __forceinline__ int count(int xcd) const { return q + (xcd < r ? 1 : 0); }
-  __device__ __forceinline__ int first(int xcd) const { return xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q; }
-  __device__ __forceinline__ void at(int t, int& ia, int& ib) const {
-    const int per = 8 * b, grp = t / per, a0 = grp * 8, wdt = min(8, a - a0), rem = t - grp * per;
-    ia = a0 + rem % wdt;
-    ib = rem / wdt;
-  }
-};
-
 template <typename C>
 __device__ __forceinline__ void dlogits_body(const LossArgs& a, char* smem) {
   const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
-  const int n = *a.count;
-  const Order2 O((n + C::BM - 1) / C::BM, a.piece / C::BN);
-  const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3, slots = gridDim.x >> 3;
-  const int cnt = O.count(xcd), base = O.first(xcd);
-  if (slot >= cnt) return;
+  const Order O(*a.count, a.piece, C::BM, C::BN, gridDim.x, blockIdx.x & 7);
+  Walk L(O, blockIdx.x >> 3), A = L, M = L;      // operands, words, sums
+  const int tiles = M.left(O);
+  if (tiles == 0) return;
   const float cs = a.inv_t * LOG2E;
-  const int lkp = 31 - __builtin_clz((unsigned)a.kp);
-  float* slab = vg_slab<C>(smem, wave);
-  vg_run<C, false, false>(
-      (cnt - slot + slots - 1) / slots, smem,
-      [&](int i, VgOperand& X, VgOperand& W, int& k0, int& k1) {
-        int tm, tn;
-        O.at(base + slot + i * slots, tm, tn);
-        const int n0 = a.v0 + tn * C::BN;
-        X = VgOperand{a.hc + (int64_t)tm * C::BM * a.hp, a.hp, C::BM, a.hp};
+  const bool label = !a.topk;
+  char* slab = smem + C::O_SLAB + wave * C::SLAB;
+  vg_run<C, false, false, true>(
+      tiles, smem,
+      [&](int, int& k0, int& k1) { k0 = 0; k1 = a.hp / VG_K; },
+      [&](int, VgOperand& X, VgOperand& W) {
+        const int n0 = a.v0 + L.vt * C::BN;
+        X = VgOperand{a.hc + (int64_t)L.rb * C::BM * a.hp, a.hp, C::BM, a.hp};
         W = VgOperand{a.weight + (int64_t)min(n0, a.vocab - 1) * a.ld_w, a.ld_w, max(1, a.vocab - n0), a.dim};
-        k0 = 0;
-        k1 = a.hp / VG_K;
+        L.next(O);
       },
-      [&](int i, f32x4 (&acc)[C::MI][C::NI]) {
-        int tm, tn;
-        O.at(base + slot + i * slots, tm, tn);
+      [&](int, char* w) {
+        Words<C>::bring(a, a.v0 + A.vt * C::BN, (int64_t)A.rb * C::BM, true, w);
+        A.next(O);
+      },
+      [&](int, f32x4 (&acc)[C::MI][C::NI], char* w) { Words<C>::start(a, a.v0 + M.vt * C::BN, wn, lq, w, acc); },
+      [&](int, f32x4 (&acc)[C::MI][C::NI], char* w) {
+        const int tm = M.rb, tn = M.vt;
+        M.next(O);
         const int64_t m0 = (int64_t)tm * C::BM + wm * 16 * C::MI;
         const int c0 = tn * C::BN + wn * 16 * C::NI;                  // the wave's first column in the piece
-        const int v0 = a.v0 + c0;
-        float b2[C::NI][4];
+        const int n0 = a.v0 + c0 + lq * 4;                            // this lane's columns: n0 + j * 16 + e
+        f32x4 col[C::NI];
 #pragma unroll
-        for (int j = 0; j < C::NI; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int v = v0 + j * 16 + lq * 4 + e;
-            b2[j][e] = v < a.vocab && a.bias ? a.bias[v] * cs : 0.f;
-          }
-        constexpr int LPR = C::SLAB_COLS / 8, RPP = 64 / LPR;         // lanes per row on the way out, rows per pass
-        float col[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) col[e] = 0.f;
+        for (int j = 0; j < C::NI; ++j) col[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int q = 0; q < C::MI; ++q) {
-          const int64_t r0 = m0 + q * 16;
-          const float lse2 = r0 + l16 < n ? a.lse2[r0 + l16] : 0.f, g = r0 + l16 < n ? a.g[r0 + l16] : 0.f;
+          const int row = (wm * C::MI + q) * 16 + l16;
+          const float nl = -*reinterpret_cast<const float*>(w + Words<C>::LSE + row * 4), g = *reinterpret_cast<const float*>(w + Words<C>::G + row * 4);
+          f32x4 p[C::NI];
+#pragma unroll
+          for (int j = 0; j < C::NI; ++j) p[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (g != 0.f) {      // a row of weight 0 has no gradient, whatever its logits are
+#pragma unroll
+            for (int j = 0; j < C::NI; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) p[j][e] = g * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[q][j][e], cs, nl));
+            if (label) {
+              const int d = *reinterpret_cast<const int*>(w + Words<C>::Y + row * 4) - n0;
+              if ((unsigned)d < 16u * C::NI && (d & 12) == 0) {
+#pragma unroll
+                for (int j = 0; j < C::NI; ++j)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    if (d == j * 16 + e) p[j][e] -= g;
+              }
+            }
+          }
 #pragma unroll
           for (int j = 0; j < C::NI; ++j) {
-            f32x4 p;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = g * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[q][j][e], cs, b2[j][e]) - lse2);
-              p[e] = g != 0.f && v0 + j * 16 + lq * 4 + e < a.vocab ? x : 0.f;      // a row of weight 0 has no gradient, whatever its logits are
-            }
-            *reinterpret_cast<f32x4*>(slab + vg_slab_at<C>(l16, j * 4 + lq)) = p;
+            col[j] += p[j];
+            vg_slab_put<C>(slab, l16, lq, j, p[j]);
           }
           CACO_WAVE_LDS_SYNC();
-          // the targets of these 16 rows that fall into the wave's columns (indices of one row are distinct)
-          for (int t = lane; t < 16 << lkp; t += 64) {
-            const int64_t r = r0 + (t >> lkp);
-            const int c = a.tgt_idx[(r0 << lkp) + t] - v0;
-            if ((unsigned)c < (unsigned)C::SLAB_COLS && r < n) {
-              const float gr = a.g[r];
-              if (gr != 0.f) slab[vg_slab_at<C>(t >> lkp, c >> 2) + (c & 3)] -= gr * a.tgt_q[(r0 << lkp) + t];
-            }
-          }
-          CACO_WAVE_LDS_SYNC();
-#pragma unroll
-          for (int ps = 0; ps < 16 / RPP; ++ps) {
-            const int row = ps * RPP + lane / LPR, ch = (lane % LPR) * 2;
-            const f32x4 u = *reinterpret_cast<const f32x4*>(slab + vg_slab_at<C>(row, ch)), v = *reinterpret_cast<const f32x4*>(slab + vg_slab_at<C>(row, ch + 1));
-            bf16x8 o;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              o[e] = (bf16_t)u[e];
-              o[e + 4] = (bf16_t)v[e];
-              col[e] += u[e];
-              col[e + 4] += v[e];
-            }
-            *reinterpret_cast<bf16x8*>(a.dl + (r0 + row) * a.piece + c0 + ch * 4) = o;
-          }
+          vg_slab_rows<C>(slab, lane, [&](int r, int ch, bf16x8 v) { *reinterpret_cast<bf16x8*>(a.dl + (m0 + q * 16 + r) * a.piece + c0 + ch * 8) = v; });
           CACO_WAVE_LDS_SYNC();
         }
         if (a.db) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
+          for (int j = 0; j < C::NI; ++j)
 #pragma unroll
-            for (int o = LPR; o < 64; o <<= 1) col[e] += __shfl_xor(col[e], o, 64);
-          if (lane < LPR) {
-            float* d = a.dbp + ((int64_t)tm * C::WM + wm) * a.piece + c0 + lane * 8;
+            for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) d[e] = col[e];
-          }
+              for (int o = 1; o < 16; o <<= 1) col[j][e] += __shfl_xor(col[j][e], o, 64);
+          if (l16 == 0)
+#pragma unroll
+            for (int j = 0; j < C::NI; ++j) *reinterpret_cast<f32x4*>(a.dbp + ((int64_t)tm * C::WM + wm) * a.piece + c0 + j * 16 + lq * 4) = col[j];
         }
       });
 }
@@ -524,141 +616,177 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
   dlogits_body<C>(a, smem);
 }
 
+// exponent e of the fixed point: every |g| < 2^e (0 where none is finite and positive: nothing is added then, or NaN reaches the sums anyway)
+__device__ __forceinline__ int fixed_exponent(const LossArgs& a) {
+  const unsigned m = *a.gmax;
+  return m == 0 || m >= 0x7f800000u ? 0 : max((int)(m >> 23), 1) - 126;
+}
+
+// (distillation) d logits at the teacher's tokens of the piece: one thread per entry.  The tokens of a row are distinct, so an entry is
+// written by one thread.  Their share of d bias is added as 64-bit integers, whose sum does not depend on the order: an entry is below
+// 2^38 units (q <= 1), the 2^24 rows' sum below 2^62, and a unit is 2^-38 of the largest |g|.
+__global__ __launch_bounds__(256) void targets2_kernel(LossArgs a) {
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t c = t / a.kp;
+  if (c >= *a.count) return;
+  const int idx = a.tgt_idx[t], v = idx - a.v0;
+  const float g = a.g[c], q = a.tgt_q[t];
+  if (idx < 0 || v < 0 || v >= a.piece || g == 0.f || q == 0.f) return;
+  a.dl[c * a.piece + v] = (bf16_t)(g * __builtin_amdgcn_exp2f(a.tgt_z[t] - a.lse2[c]) - g * q);
+  if (!a.db) return;
+  const float x = ldexpf(g * q, 38 - fixed_exponent(a));
+  if (fabsf(x) <= 0x1p38f) atomicAdd(a.db64 + idx, (unsigned long long)(long long)rintf(x));
+}
+
 __global__ __launch_bounds__(256) void dbias_kernel(LossArgs a, int bm, int wm) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= a.piece || a.v0 + c >= a.vocab) return;
   const int parts = (*a.count + bm - 1) / bm * wm;
   float s = 0.f;
   for (int p = 0; p < parts; ++p) s += a.dbp[(int64_t)p * a.piece + c];
+  if (a.topk) s -= (float)ldexp((double)(long long)a.db64[a.v0 + c], fixed_exponent(a) - 38);
   a.db[a.v0 + c] = s;
 }
 
-// d hidden of the piece: (row block, column block, slab) units, the piece's K-tiles split evenly over the slabs
-struct DhUnits {
-  int rb, cb, slabs, units;
-  __device__ __forceinline__ DhUnits(int n, int dim, int piece, int bm, int bn) {
-    rb = (n + bm - 1) / bm;
-    cb = (dim + bn - 1) / bn;
-    slabs = rb > 0 ? max(1, min(piece / VG_K, DH_UNITS / (rb * cb))) : 1;
-    units = rb * cb * slabs;
+// How a piece's gradient work is shared out.  d weight: whole tiles, an XCD a run of them, its workgroups one after the other.  d hidden:
+// the K-tiles of all its output tiles in one list, cut into a run per workgroup so that every workgroup has the same number of K-tiles in
+// all.  A run's part of an output tile is kept at [tile + workgroup] (the pair grows with every such part, so the places are distinct).
+struct Share {
+  int rb, cb, nk;                  // d hidden: row blocks, column blocks, K-tiles of an output tile
+  int wt, nkw, f;                  // d weight: tiles, K-tiles of each, tiles that every workgroup has
+  int slots;                       // workgroups of an XCD
+  int64_t total;                   // K-tiles of d hidden
+  int64_t few, many;               // d hidden K-tiles of a workgroup with one more d weight tile, and with one less
+  __device__ __forceinline__ Share(const LossArgs& a, int n, int wgs) {
+    rb = a.dh ? (n + 255) / 256 : 0;
+    cb = (a.dim + 255) / 256;
+    nk = a.piece / VG_K;
+    wt = a.dw ? a.piece / 256 * cb : 0;
+    nkw = (n + VG_K - 1) / VG_K;
+    slots = wgs / 8;
+    total = (int64_t)rb * cb * nk;
+    // f * wgs + x tiles: x workgroups have f + 1 of them.  all = K-tiles of everything, shared evenly if no workgroup has more already
+    f = wt / wgs;
+    const int x = wt % wgs;
+    const int64_t all = total + (int64_t)wt * nkw;
+    few = max((int64_t)0, (all + wgs - 1) / wgs - (int64_t)(f + 1) * nkw);
+    many = max((int64_t)0, (total - few * x + (wgs - x) - 1) / (wgs - x));
+  }
+  __device__ __forceinline__ int tiles_of(int xcd) const { return (wt >> 3) + (xcd < (wt & 7) ? 1 : 0); }
+  __device__ __forceinline__ int first_tile(int xcd) const { return xcd * (wt >> 3) + min(xcd, wt & 7); }
+  // first K-tile of workgroup w (XCD-major): of an XCD's workgroups the first ones have a d weight tile more
+  __device__ __forceinline__ int64_t first(int w) const {
+    const int xcd = w / slots, s = w % slots;
+    if (xcd >= 8) return total;
+    int64_t at = 0;
+    for (int y = 0; y <= xcd; ++y) {
+      const int in = y < xcd ? slots : s, more = min(tiles_of(y) - f * slots, in);
+      at += more * few + (in - more) * many;
+    }
+    return min(at, total);
   }
 };
-template <typename C>
-__device__ __forceinline__ void dhidden_body(const LossArgs& a, int first_piece, int full_piece, char* smem) {
+
+__device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
+  typedef Big C;
   const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
   const int n = *a.count;
-  const DhUnits U(n, a.dim, full_piece, C::BM, C::BN);
-  const int wg = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-  if (wg >= U.units) return;
-  const int nk = a.piece / VG_K;
-  vg_run<C, false, true>(
-      (U.units - wg + gridDim.x - 1) / gridDim.x, smem,
-      [&](int i, VgOperand& X, VgOperand& W, int& k0, int& k1) {
-        const int u = wg + i * gridDim.x, cb = u % U.cb, rest = u / U.cb, rb = rest % U.rb, s = rest / U.rb;
-        k0 = (int)((int64_t)s * nk / U.slabs);
-        k1 = (int)((int64_t)(s + 1) * nk / U.slabs);
+  const Share S(a, n, gridDim.x);
+  const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3, wg = xcd * S.slots + slot;
+  char* slab = smem + C::O_SLAB + wave * C::SLAB;
+  // d weight: both operands with the token slowest.  Column blocks fastest: they share a panel of d logits
+  const int cnt = S.tiles_of(xcd), base = S.first_tile(xcd);
+  if (slot < cnt)
+    vg_run<C, true, true, false>(
+        (cnt - slot + S.slots - 1) / S.slots, smem,
+        [&](int, int& k0, int& k1) { k0 = 0; k1 = S.nkw; },
+        [&](int i, VgOperand& X, VgOperand& W) {
+          const int t = base + slot + i * S.slots, tn = t % S.cb, tm = t / S.cb;
+          X = VgOperand{a.dl + tm * C::BM, a.piece, C::BM, (int64_t)S.nkw * VG_K};
+          W = VgOperand{a.hc + tn * C::BN, a.hp, a.hp - tn * C::BN, (int64_t)S.nkw * VG_K};
+        },
+        VgNoAux{}, VgZero{},
+        [&](int i, f32x4 (&acc)[C::MI][C::NI], char*) {
+          const int t = base + slot + i * S.slots, tn = t % S.cb, tm = t / S.cb;
+          const int v0 = a.v0 + tm * C::BM + wm * 16 * C::MI, c0 = tn * C::BN + wn * 16 * C::NI;
+#pragma unroll
+          for (int q = 0; q < C::MI; ++q) {
+#pragma unroll
+            for (int j = 0; j < C::NI; ++j) vg_slab_put<C>(slab, l16, lq, j, acc[q][j]);
+            CACO_WAVE_LDS_SYNC();
+            vg_slab_rows<C>(slab, lane, [&](int r, int ch, bf16x8 v) {
+              const int vv = v0 + q * 16 + r, cc = c0 + ch * 8;
+              if (vv < a.vocab && cc < a.dim) *reinterpret_cast<bf16x8*>(a.dw + (int64_t)vv * a.ld_dw + cc) = v;
+            });
+            CACO_WAVE_LDS_SYNC();
+          }
+        });
+  // d hidden: this workgroup's run, one part per output tile it touches
+  const int64_t f0 = S.first(wg), f1 = S.first(wg + 1);
+  if (f0 >= f1) return;
+  const int o0 = (int)(f0 / S.nk);
+  const bool first_piece = a.v0 == 0;
+  vg_run<C, false, true, false>(
+      (int)((f1 - 1) / S.nk) - o0 + 1, smem,
+      [&](int i, int& k0, int& k1) {
+        k0 = (int)max((int64_t)0, f0 - (int64_t)(o0 + i) * S.nk);
+        k1 = (int)min((int64_t)S.nk, f1 - (int64_t)(o0 + i) * S.nk);
+      },
+      [&](int i, VgOperand& X, VgOperand& W) {
+        const int o = o0 + i, cb = o % S.cb, rb = o / S.cb;
         X = VgOperand{a.dl + (int64_t)rb * C::BM * a.piece, a.piece, C::BM, a.piece};
         W = VgOperand{a.weight + (int64_t)a.v0 * a.ld_w + cb * C::BN, a.ld_w, a.dim - cb * C::BN, a.vocab - a.v0};
       },
-      [&](int i, f32x4 (&acc)[C::MI][C::NI]) {
-        const int u = wg + i * gridDim.x, cb = u % U.cb, rest = u / U.cb, rb = rest % U.rb, s = rest / U.rb;
-        const int64_t m0 = (int64_t)rb * C::BM + wm * 16 * C::MI + l16;
-        const int c0 = cb * C::BN + wn * 16 * C::NI + lq * 4;
+      VgNoAux{}, VgZero{},
+      [&](int i, f32x4 (&acc)[C::MI][C::NI], char*) {
+        const int o = o0 + i, rb = o / S.cb;
+        float* d = a.slab + (int64_t)(o + wg) * C::BM * C::BN + (wm * 16 * C::MI + l16) * C::BN + wn * 16 * C::NI + lq * 4;
 #pragma unroll
         for (int q = 0; q < C::MI; ++q) {
-          if (m0 + q * 16 >= n) continue;
-          float* d = a.slab + ((int64_t)s * U.rb * C::BM + m0 + q * 16) * a.hs + c0;
+          if (rb * C::BM + (wm * C::MI + q) * 16 >= n) continue;
 #pragma unroll
           for (int j = 0; j < C::NI; ++j) {
-            if (c0 + j * 16 >= a.dim) continue;
             f32x4 v = acc[q][j];
-            f32x4* p = reinterpret_cast<f32x4*>(d + j * 16);
+            f32x4* p = reinterpret_cast<f32x4*>(d + q * 16 * C::BN + j * 16);
             if (!first_piece) v += *p;
             *p = v;
           }
         }
       });
 }
-template <typename C>
-__global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void dhidden_kernel(LossArgs a, int first_piece, int full_piece) {
+__global__ __launch_bounds__(Big::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void grads_kernel(LossArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  dhidden_body<C>(a, first_piece, full_piece, smem);
+  grads_body(a, smem);
 }
 
-// rows of d hidden in the caller's order: the slabs added in order and rounded once; zeros for rows that do not count
-__global__ __launch_bounds__(256) void dh_join_kernel(LossArgs a, int full_piece, int bm, int bn) {
+// rows of d hidden in the caller's order: the parts added in order and rounded once; zeros for rows that do not count
+__global__ __launch_bounds__(256) void dh_join_kernel(LossArgs a, int wgs) {
   const int64_t row = blockIdx.x;
   const int c = a.inv[row];
-  const DhUnits U(*a.count, a.dim, full_piece, bm, bn);
+  const Share S(a, *a.count, wgs);
   for (int x = threadIdx.x * 8; x < a.dim; x += 2048) {
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (c >= 0)
-      for (int s = 0; s < U.slabs; ++s) {
-        const float* p = a.slab + ((int64_t)s * U.rb * bm + c) * a.hs + x;
+    if (c >= 0) {
+      const int o = c / 256 * S.cb + x / 256;
+      // the workgroup that holds the output tile's first K-tile, then its neighbours
+      int w = 0;
+      for (int b = 256; b > 0; b >>= 1)
+        if (w + b < wgs && S.first(w + b) <= (int64_t)o * S.nk) w += b;
+      for (; w < wgs && S.first(w) < (int64_t)(o + 1) * S.nk; ++w) {
+        if (S.first(w) == S.first(w + 1)) continue;
+        const float* p = a.slab + (int64_t)(o + w) * 65536 + c % 256 * 256 + x % 256;
         const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) { v[e] += lo[e]; v[e + 4] += hi[e]; }
       }
-    bf16x8 o;
+    }
+    bf16x8 o8;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = (bf16_t)v[e];
-    *reinterpret_cast<bf16x8*>(a.dh + row * a.ld_dh + x) = o;
+    for (int e = 0; e < 8; ++e) o8[e] = (bf16_t)v[e];
+    *reinterpret_cast<bf16x8*>(a.dh + row * a.ld_dh + x) = o8;
   }
-}
-
-// the piece's rows of d weight: sums over the tokens, both operands with the token slowest
-__device__ __forceinline__ void dweight_body(const LossArgs& a, char* smem) {
-  typedef Big C;
-  const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / C::WN, wn = wave % C::WN;
-  const int n = *a.count, nk = (n + VG_K - 1) / VG_K;
-  const int cbs = (a.dim + C::BN - 1) / C::BN;
-  const Order2 O(cbs, min(a.piece, (a.vocab - a.v0 + 255) / 256 * 256) / C::BM);
-  const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3, slots = gridDim.x >> 3;
-  const int cnt = O.count(xcd), base = O.first(xcd);
-  if (slot >= cnt) return;
-  float* slab = vg_slab<C>(smem, wave);
-  vg_run<C, true, true>(
-      (cnt - slot + slots - 1) / slots, smem,
-      [&](int i, VgOperand& X, VgOperand& W, int& k0, int& k1) {
-        int tn, tm;
-        O.at(base + slot + i * slots, tn, tm);
-        X = VgOperand{a.dl + tm * C::BM, a.piece, C::BM, (int64_t)nk * VG_K};
-        W = VgOperand{a.hc + tn * C::BN, a.hp, a.hp - tn * C::BN, (int64_t)nk * VG_K};
-        k0 = 0;
-        k1 = nk;
-      },
-      [&](int i, f32x4 (&acc)[C::MI][C::NI]) {
-        int tn, tm;
-        O.at(base + slot + i * slots, tn, tm);
-        const int v0 = a.v0 + tm * C::BM + wm * 16 * C::MI;
-        const int c0 = tn * C::BN + wn * 16 * C::NI;
-        constexpr int LPR = C::SLAB_COLS / 8, RPP = 64 / LPR;
-#pragma unroll
-        for (int q = 0; q < C::MI; ++q) {
-#pragma unroll
-          for (int j = 0; j < C::NI; ++j) *reinterpret_cast<f32x4*>(slab + vg_slab_at<C>(l16, j * 4 + lq)) = acc[q][j];
-          CACO_WAVE_LDS_SYNC();
-#pragma unroll
-          for (int ps = 0; ps < 16 / RPP; ++ps) {
-            const int row = ps * RPP + lane / LPR, ch = (lane % LPR) * 2;
-            const f32x4 u = *reinterpret_cast<const f32x4*>(slab + vg_slab_at<C>(row, ch)), v = *reinterpret_cast<const f32x4*>(slab + vg_slab_at<C>(row, ch + 1));
-            bf16x8 o;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { o[e] = (bf16_t)u[e]; o[e + 4] = (bf16_t)v[e]; }
-            const int vv = v0 + q * 16 + row, cc = c0 + ch * 4;
-            if (vv < a.vocab && cc < a.dim) *reinterpret_cast<bf16x8*>(a.dw + (int64_t)vv * a.ld_dw + cc) = o;
-          }
-          CACO_WAVE_LDS_SYNC();
-        }
-      });
-}
-__global__ __launch_bounds__(Big::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void dweight_kernel(LossArgs a) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  dweight_body(a, smem);
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
@@ -669,10 +797,10 @@ int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 // Where everything lies in the workspace.  Sizes are for all `rows`; how many of them count is known on the device only.
 struct Plan {
   int64_t npad, bytes = 0;
-  int hp, hs, kp;
+  int hp, kp;
   int64_t piece;
   bool small;
-  int64_t o_count, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_hc, o_part, o_zt, o_lse2, o_g, o_dl, o_slab, o_dbp;
+  int64_t o_count, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_part, o_zt, o_lse2, o_g, o_db64, o_dl, o_slab, o_dbp;
   int64_t take(int64_t n) {
     const int64_t at = bytes;
     bytes += up(n, 256);
@@ -682,30 +810,29 @@ struct Plan {
   Plan(int64_t rows, int vocab, int dim, int topk, int64_t piece_cols) {
     npad = up(rows > 0 ? rows : 1, 256);
     hp = (int)up(dim, VG_K);
-    hs = (int)up(dim, 4);
     kp = 1;
     while (kp < topk) kp *= 2;
     small = rows <= Small::BM;
-    const int bm = small ? Small::BM : Big::BM, bn = small ? Small::BN : Big::BN;
-    o_count = take(4);
+    const int bm = small ? Small::BM : Big::BM;
+    o_count = take(8);                                         // and the largest |g|
     o_rowmap = take(npad * 4);
     o_inv = take(npad * 4);
     o_ti0 = topk ? take(npad * kp * 4) : 0;
     o_tq0 = topk ? take(npad * kp * 4) : 0;
+    o_tz = topk ? take(npad * kp * 4) : 0;
     o_ti = take(npad * kp * 4);
     o_tq = take(npad * kp * 4);
     o_hc = take(npad * hp * 2);
-    o_part = take((npad + (int64_t)MAX_WG * bm) * 8);          // slices * row blocks <= max(row blocks, workgroups)
+    o_part = take(most_groups(npad / bm) * (small ? MAX_WG : MAX_CU) * bm * 8);
     o_zt = take(npad * 4);
     o_lse2 = take(npad * 4);
     o_g = take(npad * 4);
     piece = piece_cols;
-    o_dl = o_slab = o_dbp = 0;
+    o_db64 = o_dl = o_slab = o_dbp = 0;
     if (piece) {
+      if (topk) o_db64 = take((int64_t)vocab * 8);
       o_dl = take(npad * piece * 2);
-      const int64_t tiles = up(npad, bm) / bm * ((dim + bn - 1) / bn);
-      // slabs * row blocks * BM rows of hs columns; slabs * row blocks * column blocks <= max(DH_UNITS, tiles)
-      o_slab = take((tiles > DH_UNITS ? tiles : DH_UNITS) / ((dim + bn - 1) / bn) * bm * hs * 4);
+      o_slab = take((npad / 256 * ((dim + 255) / 256) + MAX_CU) * 65536 * 4);
       o_dbp = take(npad / bm * (small ? Small::WM : Big::WM) * piece * 4);
     }
   }
@@ -729,30 +856,28 @@ int launch(const char* what, K kern, dim3 grid, int threads, int lds, hipStream_
 }
 
 template <typename C>
-int run_loss(LossArgs& a, const Plan& P, int what, int wgs, hipStream_t st) {
+int run_loss(LossArgs& a, const Plan& P, int what, int cus, hipStream_t st) {
   const dim3 rows4((unsigned)((a.rows + 3) / 4));
   const dim3 pad4((unsigned)(P.npad / 4));
+  const int wgs = P.small ? 2 * cus : cus;
+  const bool fwd = what & CACO_LOSS_FORWARD, bwd = what & CACO_LOSS_BACKWARD;
   if (a.topk && a.rows) CACO_TRY_RC(launch("loss targets", targets_kernel, rows4, 256, 0, st, a));
   CACO_TRY_RC(launch("loss compact", compact_kernel, dim3(1), 1024, 0, st, a));
-  CACO_TRY_RC(launch("loss gather", gather_kernel, pad4, 256, 0, st, a, (what & CACO_LOSS_BACKWARD) != 0, (what & CACO_LOSS_FORWARD) == 0));
-  if (what & CACO_LOSS_FORWARD) {
-    if (a.topk) CACO_TRY_RC(launch("loss target logits", target_logits_kernel, pad4, 256, 0, st, a));
+  CACO_TRY_RC(launch("loss gather", gather_kernel, pad4, 256, 0, st, a, (int)bwd, (int)!fwd));
+  if (a.topk) CACO_TRY_RC(launch("loss target logits", target_logits_kernel, pad4, 256, 0, st, a));
+  if (fwd) {
     CACO_TRY_RC(launch("loss lse", lse_kernel<C>, dim3(wgs), C::THREADS, C::SMEM, st, a));
     if (a.rows) CACO_TRY_RC(launch("loss finish", finish_kernel, rows4, 256, 0, st, a, (int)C::BM, (int)C::BN, wgs));
     if (a.loss) CACO_TRY_RC(launch("loss reduce", reduce_kernel, dim3(1), 1024, 0, st, a));
   }
-  if (!(what & CACO_LOSS_BACKWARD)) return CACO_OK;
-  const int full = a.piece;
-  int num_cu = 0;
-  CACO_TRY_RC(prepare_launch(reinterpret_cast<const void*>(&dweight_kernel), Big::SMEM, &num_cu));
-  for (int v0 = 0; v0 < a.vocab; v0 += full) {
-    a.v0 = v0;
+  if (!bwd) return CACO_OK;
+  for (; a.v0 < a.vocab; a.v0 += a.piece) {
     CACO_TRY_RC(launch("loss dlogits", dlogits_kernel<C>, dim3(wgs), C::THREADS, C::SMEM, st, a));
+    if (a.topk) CACO_TRY_RC(launch("loss targets2", targets2_kernel, dim3((unsigned)(P.npad * a.kp / 256)), 256, 0, st, a));
     if (a.db) CACO_TRY_RC(launch("loss dbias", dbias_kernel, dim3((a.piece + 255) / 256), 256, 0, st, a, (int)C::BM, (int)C::WM));
-    if (a.dh) CACO_TRY_RC(launch("loss dhidden", dhidden_kernel<C>, dim3(wgs), C::THREADS, C::SMEM, st, a, v0 == 0, full));
-    if (a.dw) CACO_TRY_RC(launch("loss dweight", dweight_kernel, dim3(num_cu / 8 * 8), Big::THREADS, Big::SMEM, st, a));
+    if (a.dh || a.dw) CACO_TRY_RC(launch("loss grads", grads_kernel, dim3(cus), Big::THREADS, Big::SMEM, st, a));
   }
-  if (a.dh && a.rows) CACO_TRY_RC(launch("loss dhidden join", dh_join_kernel, dim3((unsigned)a.rows), 256, 0, st, a, full, (int)C::BM, (int)C::BN));
+  if (a.dh && a.rows) CACO_TRY_RC(launch("loss dhidden join", dh_join_kernel, dim3((unsigned)a.rows), 256, 0, st, a, cus));
   return CACO_OK;
 }
 
@@ -762,6 +887,7 @@ int check_sizes(int64_t rows, int32_t vocab, int32_t dim, int32_t topk) {
   CACO_REQUIRE(rows >= 0 && rows <= (int64_t)1 << 24, "linear loss: rows must be 0 .. 2^24, got %lld", (long long)rows);
   CACO_REQUIRE(vocab >= 1 && vocab <= 1 << 24, "linear loss: vocab must be 1 .. 2^24, got %d", vocab);
   CACO_REQUIRE(dim >= 8 && dim <= 1 << 16 && dim % 8 == 0, "linear loss: dim must be a multiple of 8 in 8 .. 65536, got %d", dim);
+  CACO_REQUIRE(up(rows, 256) * up(vocab, 256) <= (int64_t)1 << 46, "linear loss: rows * vocab must not exceed 2^46, got %lld * %d", (long long)rows, vocab);
   CACO_REQUIRE(topk >= 0 && topk <= 128, "linear loss: topk must be 1 .. 128, got %d", topk);
   return CACO_OK;
 }
@@ -814,22 +940,23 @@ int linear_loss(const LinearLoss& c, hipStream_t st) {
   a.topk = c.topk; a.kp = P.kp;
   a.temperature = c.topk ? c.temperature : 1.f;
   a.inv_t = 1.f / a.temperature;
-  a.rows = c.rows; a.vocab = c.vocab; a.dim = c.dim; a.hp = P.hp; a.hs = P.hs;
+  a.rows = c.rows; a.vocab = c.vocab; a.dim = c.dim; a.hp = P.hp;
   a.reduction = c.reduction; a.row_weight = c.row_weight; a.grad_scale = c.grad_scale;
   a.row_loss = c.row_loss; a.lse = c.lse; a.loss = c.loss;
   a.dh = bwd ? c.d_hidden : nullptr; a.ld_dh = c.ld_dh; a.dw = bwd ? c.d_weight : nullptr; a.ld_dw = c.ld_dw; a.db = bwd ? c.d_bias : nullptr;
   char* w = reinterpret_cast<char*>(c.ws);
   a.count = (int*)(w + P.o_count); a.rowmap = (int*)(w + P.o_rowmap); a.inv = (int*)(w + P.o_inv);
   a.tgt_idx0 = (int*)(w + P.o_ti0); a.tgt_q0 = (float*)(w + P.o_tq0); a.tgt_idx = (int*)(w + P.o_ti); a.tgt_q = (float*)(w + P.o_tq);
-  a.hc = (bf16_t*)(w + P.o_hc); a.part = (float2*)(w + P.o_part); a.zt = (float*)(w + P.o_zt); a.lse2 = (float*)(w + P.o_lse2); a.g = (float*)(w + P.o_g);
+  a.hc = (bf16_t*)(w + P.o_hc); a.part = (float2*)(w + P.o_part); a.zt = (float*)(w + P.o_zt); a.tgt_z = (float*)(w + P.o_tz); a.lse2 = (float*)(w + P.o_lse2); a.g = (float*)(w + P.o_g);
   a.dl = (bf16_t*)(w + P.o_dl); a.slab = (float*)(w + P.o_slab); a.dbp = (float*)(w + P.o_dbp);
+  a.gmax = (unsigned*)(a.count + 1); a.db64 = (unsigned long long*)(w + P.o_db64);
   a.piece = (int)piece;
   int num_cu = 0;
   CACO_TRY_RC(prepare_launch(reinterpret_cast<const void*>(&lse_kernel<Big>), Big::SMEM, &num_cu));
-  const int cus = num_cu / 8 * 8 < 8 ? 8 : num_cu / 8 * 8;
-  const int wgs = P.small ? 2 * cus : cus;
-  CACO_REQUIRE(wgs <= MAX_WG, "linear loss: %d compute units", num_cu);
-  return P.small ? run_loss<Small>(a, P, c.what, wgs, st) : run_loss<Big>(a, P, c.what, wgs, st);
+  // a power of two of workgroups per XCD, 8 at least (Order)
+  int cus = 64;
+  while (cus * 2 <= num_cu && cus < MAX_CU) cus *= 2;
+  return P.small ? run_loss<Small>(a, P, c.what, cus, st) : run_loss<Big>(a, P, c.what, cus, st);
 }
 
 }  // namespace caco

@@ -210,7 +210,7 @@ void caco_decode_end(caco_decode_state* s);
  *   unless the forward pass is part of the same call (CACO_LOSS_FORWARD | CACO_LOSS_BACKWARD).  No row counts: zero gradients.
  *   row_weight_dev fp32 [rows] or NULL (= 1), grad_scale_dev fp32 [1] or NULL (= 1).
  * Row strides are in elements, >= dim and multiples of 8, and rows start at multiples of 16 bytes; dim is a multiple of 8; rows <= 2^24
- *   (0 is allowed), vocab <= 2^24, dim <= 65536.
+ *   (0 is allowed), vocab <= 2^24, rows * vocab <= 2^46 (both rounded up to 256), dim <= 65536.
  * ws_dev: scratch of the caller's, 16-byte aligned, its contents are not kept; one call at a time may use it.  caco_linear_loss_workspace
  *   gives its size (topk 0 = cross entropy; < 0: CACO_ERR_INVALID); with the backward pass it includes the gradient of the logits
  *   for one piece of the vocabulary in bf16, of about piece_bytes (at least 256 columns).  A smaller workspace makes more pieces.

@@ -216,6 +216,13 @@ static inline void __builtin_amdgcn_s_barrier() { wavesim::block_barrier(); }
 static inline void __syncthreads() { wavesim::vm_wait(0); wavesim::block_barrier(); }
 static inline int __syncthreads_or(int pred) { wavesim::vm_wait(0); return wavesim::block_barrier_or(pred); }
 
+static inline unsigned long long atomicAdd(unsigned long long* p, unsigned long long v) { return __atomic_fetch_add(p, v, __ATOMIC_RELAXED); }
+static inline unsigned atomicMax(unsigned* p, unsigned v) {
+  unsigned o = __atomic_load_n(p, __ATOMIC_RELAXED);
+  while (o < v && !__atomic_compare_exchange_n(p, &o, v, false, __ATOMIC_RELAXED, __ATOMIC_RELAXED)) {}
+  return o;
+}
+static inline unsigned __float_as_uint(float f) { unsigned u; memcpy(&u, &f, 4); return u; }
 template <typename T>
 static inline T wavesim_exchange_from(T v, int src_lane, const void* site) {
   static_assert(sizeof(T) <= 8, "shuffle payload");
