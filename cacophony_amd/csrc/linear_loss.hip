@@ -67,7 +67,7 @@ struct LossArgs {
   float* zt;                         // cross entropy: the label's log2-logit; distillation: sum_k q_k (z_k / T - log q_k), log2 units
   float* tgt_z;                      // distillation: the entries' log2-logits [npad, kp]
   float *lse2, *g;                   // compact: lse in log2 units, gradient scale of the row
-  unsigned* gmax;                    // bits of the largest |g|
+  float* wmax;                       // largest |row_weight| of the rows that count
   unsigned long long* db64;          // distillation: sum of the targets' weights per word, fixed point in units of 2^(e - 38), |g| < 2^e
   bf16_t* dl;                        // [npad, piece]
   float* slab;                       // d hidden's partial sums [output tile + workgroup][256][256]
@@ -145,8 +145,10 @@ __device__ __forceinline__ bool row_counts(const LossArgs& a, int64_t r) {
 }
 
 // One workgroup: every thread counts a run of consecutive rows, a scan over the threads gives each run its first place.
+// Also the largest |row_weight| of the rows that count.
 __global__ __launch_bounds__(1024) void compact_kernel(LossArgs a) {
   __shared__ int s_wave[16];
+  __shared__ float s_max[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t per = (a.rows + 1023) / 1024;
   const int64_t r0 = min(a.rows, tid * per), r1 = min(a.rows, r0 + per);
@@ -161,16 +163,32 @@ __global__ __launch_bounds__(1024) void compact_kernel(LossArgs a) {
   if (lane == 63) s_wave[wave] = incl;
   __syncthreads();
   int at = incl - n;
+  float wmax = a.row_weight ? 0.f : 1.f;
   for (int w = 0; w < wave; ++w) at += s_wave[w];
   for (int64_t r = r0; r < r1; ++r) {
     const bool c = row_counts(a, r);      // this thread's own rows: read before they are overwritten
     a.inv[r] = c ? at : -1;
-    if (c) a.rowmap[at++] = (int)r;
+    if (c) {
+      a.rowmap[at++] = (int)r;
+      if (a.row_weight) wmax = fmaxf(wmax, fabsf(a.row_weight[r]));
+    }
   }
-  if (tid == 1023) {
-    *a.count = at;
-    *a.gmax = 0;
+  wmax = wave_max(wmax);
+  if (lane == 0) s_max[wave] = wmax;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < 16; ++w) wmax = fmaxf(wmax, s_max[w]);
+    *a.wmax = wmax;
   }
+  if (tid == 1023) *a.count = at;
+}
+
+// T from the logits' scale and the loss's T^2, the row's weight, the incoming gradient, the mean
+__device__ __forceinline__ float row_gradient(const LossArgs& a, float weight, int n) {
+  float g = a.temperature * weight;
+  if (a.grad_scale) g *= *a.grad_scale;
+  if (a.reduction == CACO_REDUCE_MEAN) g /= (float)n;
+  return g;
 }
 
 // compact row <- its hidden state, targets, gradient scale.  One wave per row; rows up to the next multiple of 256 are zero rows.
@@ -197,12 +215,7 @@ __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, i
     a.tgt_q[c * a.kp + k] = q;
   }
   if (backward && lane == 0) {
-    float g = real ? a.temperature : 0.f;
-    if (real && a.row_weight) g *= a.row_weight[row];
-    if (real && a.grad_scale) g *= *a.grad_scale;
-    if (real && a.reduction == CACO_REDUCE_MEAN) g /= (float)n;
-    a.g[c] = g;
-    atomicMax(a.gmax, __float_as_uint(fabsf(g)));      // a maximum does not depend on the order
+    a.g[c] = real ? row_gradient(a, a.row_weight ? a.row_weight[row] : 1.f, n) : 0.f;
     if (from_lse) a.lse2[c] = real ? a.lse[row] * LOG2E : 0.f;
   }
 }
@@ -616,9 +629,9 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
   dlogits_body<C>(a, smem);
 }
 
-// exponent e of the fixed point: every |g| < 2^e (0 where none is finite and positive: nothing is added then, or NaN reaches the sums anyway)
+// exponent e of the fixed point: every |g| < 2^e, because row_gradient grows with |weight| (0 where the largest is not finite or is zero)
 __device__ __forceinline__ int fixed_exponent(const LossArgs& a) {
-  const unsigned m = *a.gmax;
+  const unsigned m = __float_as_uint(fabsf(row_gradient(a, *a.wmax, *a.count)));
   return m == 0 || m >= 0x7f800000u ? 0 : max((int)(m >> 23), 1) - 126;
 }
 
@@ -648,42 +661,61 @@ __global__ __launch_bounds__(256) void dbias_kernel(LossArgs a, int bm, int wm) 
   a.db[a.v0 + c] = s;
 }
 
-// How a piece's gradient work is shared out.  d weight: whole tiles, an XCD a run of them, its workgroups one after the other.  d hidden:
-// the K-tiles of all its output tiles in one list, cut into a run per workgroup so that every workgroup has the same number of K-tiles in
-// all.  A run's part of an output tile is kept at [tile + workgroup] (the pair grows with every such part, so the places are distinct).
+// How a piece's gradient work is shared out, XCD by XCD.
+//   d weight   an XCD takes a run of whole tiles, its workgroups one after the other, column blocks fastest: they share a panel of d logits.
+//   d hidden   `ks` slices of the vocabulary times 8 / ks runs of the output tiles: the fewest slices that leave an XCD a tile for each of its
+//              workgroups, so that these walk the same part of the vocabulary together, with few panels between them (at 22 row blocks and
+//              3 column blocks 0.4 MB per K-tile instead of 2 MB, which the XCD's L2 then holds).  Tiles beyond a multiple of the
+//              workgroups make one list of K-tiles, cut so that workgroups with one d weight tile less get more of it.
+// A slice of a whole tile is kept at [tile][slice], a part of the list at [XCD][tile of the list + workgroup] (the sum grows from part to
+// part, so the places are distinct).
 struct Share {
-  int rb, cb, nk;                  // d hidden: row blocks, column blocks, K-tiles of an output tile
-  int wt, nkw, f;                  // d weight: tiles, K-tiles of each, tiles that every workgroup has
-  int slots;                       // workgroups of an XCD
-  int64_t total;                   // K-tiles of d hidden
-  int64_t few, many;               // d hidden K-tiles of a workgroup with one more d weight tile, and with one less
-  __device__ __forceinline__ Share(const LossArgs& a, int n, int wgs) {
+  int rb, cb, tiles, nk, ks;       // d hidden: row blocks, column blocks, output tiles, K-tiles of one, slices
+  int nkw, slots;                  // d weight: K-tiles of a tile; workgroups of an XCD
+  int wcnt, wbase;                 // this XCD's d weight tiles, the first
+  int slice, k0, nkx;              // its slice, the slice's first K-tile and length
+  int t0, whole, rest;             // its output tiles: the first, whole ones per workgroup, tiles in the list
+  int more, few, many;             // workgroups with a d weight tile more; K-tiles of the list for these and for the others
+  __device__ __forceinline__ Share(const LossArgs& a, int n, int wgs, int xcd) {
+    slots = wgs >> 3;
     rb = a.dh ? (n + 255) / 256 : 0;
     cb = (a.dim + 255) / 256;
+    tiles = rb * cb;
     nk = a.piece / VG_K;
-    wt = a.dw ? a.piece / 256 * cb : 0;
     nkw = (n + VG_K - 1) / VG_K;
-    slots = wgs / 8;
-    total = (int64_t)rb * cb * nk;
-    // f * wgs + x tiles: x workgroups have f + 1 of them.  all = K-tiles of everything, shared evenly if no workgroup has more already
-    f = wt / wgs;
-    const int x = wt % wgs;
-    const int64_t all = total + (int64_t)wt * nkw;
-    few = max((int64_t)0, (all + wgs - 1) / wgs - (int64_t)(f + 1) * nkw);
-    many = max((int64_t)0, (total - few * x + (wgs - x) - 1) / (wgs - x));
+    const int wt = a.dw ? a.piece / 256 * cb : 0;
+    wcnt = (wt >> 3) + (xcd < (wt & 7) ? 1 : 0);
+    wbase = xcd * (wt >> 3) + min(xcd, wt & 7);
+    ks = slices(tiles, slots);
+    const int groups = 8 / ks, grp = xcd / ks;
+    slice = xcd % ks;
+    k0 = (int)((int64_t)slice * nk / ks);
+    nkx = (int)((int64_t)(slice + 1) * nk / ks) - k0;
+    t0 = (int)((int64_t)grp * tiles / groups);
+    const int nt = (int)((int64_t)(grp + 1) * tiles / groups) - t0;
+    whole = nt / slots;
+    rest = nt % slots;
+    const int f = wcnt / slots;
+    more = wcnt % slots;
+    const int list = rest * nkx;   // < slots * 2^18
+    few = max(0, (int)(((int64_t)list + (int64_t)wcnt * nkw + slots - 1) / slots - (int64_t)(f + 1) * nkw));
+    many = max(0, (list - (int)min((int64_t)list, (int64_t)few * more) + slots - more - 1) / (slots - more));
   }
-  __device__ __forceinline__ int tiles_of(int xcd) const { return (wt >> 3) + (xcd < (wt & 7) ? 1 : 0); }
-  __device__ __forceinline__ int first_tile(int xcd) const { return xcd * (wt >> 3) + min(xcd, wt & 7); }
-  // first K-tile of workgroup w (XCD-major): of an XCD's workgroups the first ones have a d weight tile more
-  __device__ __forceinline__ int64_t first(int w) const {
-    const int xcd = w / slots, s = w % slots;
-    if (xcd >= 8) return total;
-    int64_t at = 0;
-    for (int y = 0; y <= xcd; ++y) {
-      const int in = y < xcd ? slots : s, more = min(tiles_of(y) - f * slots, in);
-      at += more * few + (in - more) * many;
-    }
-    return min(at, total);
+  static __host__ __device__ __forceinline__ int slices(int tiles, int slots) {
+    int k = 1;
+    while (k < 8 && tiles * k < 8 * slots) k *= 2;
+    return k;
+  }
+  // first K-tile of workgroup s in the list
+  __device__ __forceinline__ int first(int s) const {
+    const int m = min(s, more);
+    return s >= slots ? rest * nkx : (int)min((int64_t)rest * nkx, (int64_t)m * few + (int64_t)(s - m) * many);
+  }
+  __device__ __forceinline__ int64_t slab_whole(int tile) const { return (int64_t)tile * ks + slice; }
+  __device__ __forceinline__ int64_t slab_list(int xcd, int i, int s) const { return (int64_t)tiles * ks + xcd * (min(tiles, slots) + slots) + i + s; }
+  // slabs that can be needed with `most` output tiles at most
+  static int64_t slabs(int64_t most, int slots) {
+    return (most > 16 * slots ? most : (most * 8 < 16 * slots ? most * 8 : 16 * slots)) + 8 * ((most < slots ? most : slots) + slots);
   }
 };
 
@@ -693,23 +725,22 @@ __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
   const int n = *a.count;
-  const Share S(a, n, gridDim.x);
-  const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3, wg = xcd * S.slots + slot;
+  const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+  const Share S(a, n, gridDim.x, xcd);
   char* slab = smem + C::O_SLAB + wave * C::SLAB;
-  // d weight: both operands with the token slowest.  Column blocks fastest: they share a panel of d logits
-  const int cnt = S.tiles_of(xcd), base = S.first_tile(xcd);
-  if (slot < cnt)
+  // d weight: both operands with the token slowest
+  if (slot < S.wcnt)
     vg_run<C, true, true, false>(
-        (cnt - slot + S.slots - 1) / S.slots, smem,
+        (S.wcnt - slot + S.slots - 1) / S.slots, smem,
         [&](int, int& k0, int& k1) { k0 = 0; k1 = S.nkw; },
         [&](int i, VgOperand& X, VgOperand& W) {
-          const int t = base + slot + i * S.slots, tn = t % S.cb, tm = t / S.cb;
+          const int t = S.wbase + slot + i * S.slots, tn = t % S.cb, tm = t / S.cb;
           X = VgOperand{a.dl + tm * C::BM, a.piece, C::BM, (int64_t)S.nkw * VG_K};
           W = VgOperand{a.hc + tn * C::BN, a.hp, a.hp - tn * C::BN, (int64_t)S.nkw * VG_K};
         },
         VgNoAux{}, VgZero{},
         [&](int i, f32x4 (&acc)[C::MI][C::NI], char*) {
-          const int t = base + slot + i * S.slots, tn = t % S.cb, tm = t / S.cb;
+          const int t = S.wbase + slot + i * S.slots, tn = t % S.cb, tm = t / S.cb;
           const int v0 = a.v0 + tm * C::BM + wm * 16 * C::MI, c0 = tn * C::BN + wn * 16 * C::NI;
 #pragma unroll
           for (int q = 0; q < C::MI; ++q) {
@@ -723,26 +754,29 @@ __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
             CACO_WAVE_LDS_SYNC();
           }
         });
-  // d hidden: this workgroup's run, one part per output tile it touches
-  const int64_t f0 = S.first(wg), f1 = S.first(wg + 1);
-  if (f0 >= f1) return;
-  const int o0 = (int)(f0 / S.nk);
+  // d hidden: the workgroup's whole tiles, then its part of the list
+  const int f0 = S.first(slot), f1 = S.first(slot + 1), l0 = f0 < f1 ? f0 / S.nkx : 0;
+  const int parts = S.whole + (f0 < f1 ? (f1 - 1) / S.nkx - l0 + 1 : 0);
+  if (parts == 0) return;
   const bool first_piece = a.v0 == 0;
+  auto out_tile = [&](int i) { return i < S.whole ? S.t0 + slot + i * S.slots : S.t0 + S.whole * S.slots + l0 + i - S.whole; };
   vg_run<C, false, true, false>(
-      (int)((f1 - 1) / S.nk) - o0 + 1, smem,
+      parts, smem,
       [&](int i, int& k0, int& k1) {
-        k0 = (int)max((int64_t)0, f0 - (int64_t)(o0 + i) * S.nk);
-        k1 = (int)min((int64_t)S.nk, f1 - (int64_t)(o0 + i) * S.nk);
+        const int at = i < S.whole ? 0 : (l0 + i - S.whole) * S.nkx;      // the tile's first K-tile in the list
+        k0 = S.k0 + (i < S.whole ? 0 : max(0, f0 - at));
+        k1 = S.k0 + (i < S.whole ? S.nkx : min(S.nkx, f1 - at));
       },
       [&](int i, VgOperand& X, VgOperand& W) {
-        const int o = o0 + i, cb = o % S.cb, rb = o / S.cb;
+        const int o = out_tile(i), cb = o % S.cb, rb = o / S.cb;
         X = VgOperand{a.dl + (int64_t)rb * C::BM * a.piece, a.piece, C::BM, a.piece};
         W = VgOperand{a.weight + (int64_t)a.v0 * a.ld_w + cb * C::BN, a.ld_w, a.dim - cb * C::BN, a.vocab - a.v0};
       },
       VgNoAux{}, VgZero{},
       [&](int i, f32x4 (&acc)[C::MI][C::NI], char*) {
-        const int o = o0 + i, rb = o / S.cb;
-        float* d = a.slab + (int64_t)(o + wg) * C::BM * C::BN + (wm * 16 * C::MI + l16) * C::BN + wn * 16 * C::NI + lq * 4;
+        const int o = out_tile(i), rb = o / S.cb;
+        const int64_t place = i < S.whole ? S.slab_whole(o) : S.slab_list(xcd, l0 + i - S.whole, slot);
+        float* d = a.slab + place * C::BM * C::BN + (wm * 16 * C::MI + l16) * C::BN + wn * 16 * C::NI + lq * 4;
 #pragma unroll
         for (int q = 0; q < C::MI; ++q) {
           if (rb * C::BM + (wm * C::MI + q) * 16 >= n) continue;
@@ -761,25 +795,45 @@ __global__ __launch_bounds__(Big::THREADS) __attribute__((amdgpu_waves_per_eu(2,
   grads_body(a, smem);
 }
 
-// rows of d hidden in the caller's order: the parts added in order and rounded once; zeros for rows that do not count
+// rows of d hidden in the caller's order, 4 to a workgroup: the parts added in order and rounded once; zeros for rows that do not count
 __global__ __launch_bounds__(256) void dh_join_kernel(LossArgs a, int wgs) {
-  const int64_t row = blockIdx.x;
+  __shared__ int s_first[8][MAX_CU / 8 + 1];
+  const int slots = wgs >> 3, n = *a.count;
+  for (int w = threadIdx.x; w < 8 * (slots + 1); w += 256) {
+    const int x = w / (slots + 1), s = w % (slots + 1);
+    s_first[x][s] = Share(a, n, wgs, x).first(s);
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.rows) return;
   const int c = a.inv[row];
-  const Share S(a, *a.count, wgs);
-  for (int x = threadIdx.x * 8; x < a.dim; x += 2048) {
+  for (int x = lane * 8; x < a.dim; x += 512) {
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (c >= 0) {
-      const int o = c / 256 * S.cb + x / 256;
-      // the workgroup that holds the output tile's first K-tile, then its neighbours
-      int w = 0;
-      for (int b = 256; b > 0; b >>= 1)
-        if (w + b < wgs && S.first(w + b) <= (int64_t)o * S.nk) w += b;
-      for (; w < wgs && S.first(w) < (int64_t)(o + 1) * S.nk; ++w) {
-        if (S.first(w) == S.first(w + 1)) continue;
-        const float* p = a.slab + (int64_t)(o + w) * 65536 + c % 256 * 256 + x % 256;
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
+      const Share S0(a, n, wgs, 0);
+      const int o = c / 256 * S0.cb + x / 256, groups = 8 / S0.ks;
+      int grp = 0;
+      while (grp + 1 < groups && (int)((int64_t)(grp + 1) * S0.tiles / groups) <= o) ++grp;
+      for (int slice = 0; slice < S0.ks; ++slice) {
+        const int xcd = grp * S0.ks + slice;
+        const Share S(a, n, wgs, xcd);
+        auto add = [&](int64_t place) {
+          const float* p = a.slab + place * 65536 + c % 256 * 256 + x % 256;
+          const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { v[e] += lo[e]; v[e + 4] += hi[e]; }
+          for (int e = 0; e < 4; ++e) { v[e] += lo[e]; v[e + 4] += hi[e]; }
+        };
+        const int i = o - S.t0 - S.whole * slots;      // its place in the list
+        if (i < 0) {
+          add(S.slab_whole(o));
+          continue;
+        }
+        int s = 0;                                       // the last workgroup that begins no later than the tile, then its neighbours
+        for (int b = MAX_CU / 8; b > 0; b >>= 1)
+          if (s + b < slots && s_first[xcd][s + b] <= i * S.nkx) s += b;
+        for (; s < slots && s_first[xcd][s] < (i + 1) * S.nkx; ++s)
+          if (s_first[xcd][s] < s_first[xcd][s + 1]) add(S.slab_list(xcd, i, s));
       }
     }
     bf16x8 o8;
@@ -814,7 +868,7 @@ struct Plan {
     while (kp < topk) kp *= 2;
     small = rows <= Small::BM;
     const int bm = small ? Small::BM : Big::BM;
-    o_count = take(8);                                         // and the largest |g|
+    o_count = take(8);                                         // and the largest weight
     o_rowmap = take(npad * 4);
     o_inv = take(npad * 4);
     o_ti0 = topk ? take(npad * kp * 4) : 0;
@@ -832,7 +886,7 @@ struct Plan {
     if (piece) {
       if (topk) o_db64 = take((int64_t)vocab * 8);
       o_dl = take(npad * piece * 2);
-      o_slab = take((npad / 256 * ((dim + 255) / 256) + MAX_CU) * 65536 * 4);
+      o_slab = take(Share::slabs(npad / 256 * ((dim + 255) / 256), MAX_CU / 8) * 65536 * 4);
       o_dbp = take(npad / bm * (small ? Small::WM : Big::WM) * piece * 4);
     }
   }
@@ -877,7 +931,7 @@ int run_loss(LossArgs& a, const Plan& P, int what, int cus, hipStream_t st) {
     if (a.db) CACO_TRY_RC(launch("loss dbias", dbias_kernel, dim3((a.piece + 255) / 256), 256, 0, st, a, (int)C::BM, (int)C::WM));
     if (a.dh || a.dw) CACO_TRY_RC(launch("loss grads", grads_kernel, dim3(cus), Big::THREADS, Big::SMEM, st, a));
   }
-  if (a.dh && a.rows) CACO_TRY_RC(launch("loss dhidden join", dh_join_kernel, dim3((unsigned)a.rows), 256, 0, st, a, cus));
+  if (a.dh && a.rows) CACO_TRY_RC(launch("loss dhidden join", dh_join_kernel, rows4, 256, 0, st, a, cus));
   return CACO_OK;
 }
 
@@ -949,7 +1003,7 @@ int linear_loss(const LinearLoss& c, hipStream_t st) {
   a.tgt_idx0 = (int*)(w + P.o_ti0); a.tgt_q0 = (float*)(w + P.o_tq0); a.tgt_idx = (int*)(w + P.o_ti); a.tgt_q = (float*)(w + P.o_tq);
   a.hc = (bf16_t*)(w + P.o_hc); a.part = (float2*)(w + P.o_part); a.zt = (float*)(w + P.o_zt); a.tgt_z = (float*)(w + P.o_tz); a.lse2 = (float*)(w + P.o_lse2); a.g = (float*)(w + P.o_g);
   a.dl = (bf16_t*)(w + P.o_dl); a.slab = (float*)(w + P.o_slab); a.dbp = (float*)(w + P.o_dbp);
-  a.gmax = (unsigned*)(a.count + 1); a.db64 = (unsigned long long*)(w + P.o_db64);
+  a.wmax = (float*)(a.count + 1); a.db64 = (unsigned long long*)(w + P.o_db64);
   a.piece = (int)piece;
   int num_cu = 0;
   CACO_TRY_RC(prepare_launch(reinterpret_cast<const void*>(&lse_kernel<Big>), Big::SMEM, &num_cu));
