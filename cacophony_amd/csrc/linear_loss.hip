@@ -69,7 +69,9 @@ struct LossArgs {
   float *lse2, *g;                   // compact: lse in log2 units, gradient scale of the row
   float* wmax;                       // largest |row_weight| of the rows that count
   unsigned long long* db64;          // distillation: sum of the targets' weights per word, fixed point in units of 2^(e - 38), |g| < 2^e
-  bf16_t* dl;                        // [npad, piece]
+  // d logits of the piece in blocks of 256 rows x 256 columns, [row block][column block][256][256]: a K-tile of either gradient is then 32 KiB
+  // next to one another or 256 rows 512 bytes apart, instead of rows a whole piece apart (100 KB at 50265 words)
+  bf16_t* dl;
   float* slab;                       // d hidden's partial sums [output tile + workgroup][256][256]
   float* dbp;                        // [row halves, piece]
   int piece, v0;                     // columns of the piece, its first column
@@ -133,6 +135,11 @@ __global__ __launch_bounds__(256) void targets_kernel(LossArgs a) {
     }
   }
   if (lane == 0) a.inv[row] = some;                        // for `compact`
+}
+
+// a row of one 256 x 256 block of d logits
+__device__ __forceinline__ bf16_t* dl_at(const LossArgs& a, int64_t row, int col) {
+  return a.dl + (((row >> 8) * (a.piece >> 8) + (col >> 8)) * 256 + (row & 255)) * 256 + (col & 255);
 }
 
 // does row r count?
@@ -318,7 +325,7 @@ template <typename C>
 struct Words {
   static constexpr int BIAS = 0, Y = C::BN * 4, LSE = Y + C::BM * 4, G = LSE + C::BM * 4;
   static __device__ __forceinline__ void bring(const LossArgs& a, int n0, int64_t m0, bool grad, char* lds) {
-    const int lane = threadIdx.x & 63;
+    const int lane = vg_lane();
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (int pc = wave; pc < (C::BN + (grad ? 3 : 1) * C::BM) / 64; pc += C::WAVES) {
       if (pc < C::BN / 64) {
@@ -332,7 +339,8 @@ struct Words {
     }
   }
   // sums begin with the bias; a column past the vocabulary with -inf, its logit and nothing else comes of it
-  static __device__ __forceinline__ void start(const LossArgs& a, int n0, int wn, int lq, const char* lds, f32x4 (&acc)[C::MI][C::NI]) {
+  static __device__ __forceinline__ void start(const LossArgs& a, int n0, int wn, const char* lds, f32x4 (&acc)[C::MI][C::NI]) {
+    const int lq = vg_lane() >> 4;
     const bool edge = n0 + C::BN > a.vocab;
 #pragma unroll
     for (int j = 0; j < C::NI; ++j) {
@@ -354,12 +362,11 @@ struct Words {
 // over the tile again with its maxima.  Logits far below the reference add what they should: nothing.
 template <typename C>
 __device__ __forceinline__ void lse_body(const LossArgs& a, char* smem) {
-  const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
   const Order O(*a.count, a.vocab, C::BM, C::BN, gridDim.x, blockIdx.x & 7);
   const int wg = (blockIdx.x & 7) * O.slots + (blockIdx.x >> 3);
-  Walk L(O, blockIdx.x >> 3), A = L, M = L;      // operands, words, sums
+  Walk L(O, blockIdx.x >> 3), M = L;      // the operands, the results
   const int tiles = M.left(O);
   if (tiles == 0) return;
   const float cs = a.inv_t * LOG2E;
@@ -367,21 +374,24 @@ __device__ __forceinline__ void lse_body(const LossArgs& a, char* smem) {
   float nref[C::MI], sm[C::MI];      // minus the reference, the sum
 #pragma unroll
   for (int q = 0; q < C::MI; ++q) { nref[q] = 3.0e38f; sm[q] = 0.f; }
-  vg_run<C, false, false, true>(
+  vg_run<C, false, false, true, true, true>(
       tiles, smem,
       [&](int, int& k0, int& k1) { k0 = 0; k1 = a.hp / VG_K; },
-      [&](int, VgOperand& X, VgOperand& W) {
+      [&](int) { return vg_rows(a.hc + (int64_t)L.rb * C::BM * a.hp, a.hp, C::BM, a.hp); },      // of the tile whose weights were asked for before
+      [&](int i) {
+        if (i > 0) L.next(O);
         const int n0 = L.vt * C::BN;
-        X = VgOperand{a.hc + (int64_t)L.rb * C::BM * a.hp, a.hp, C::BM, a.hp};
-        W = VgOperand{a.weight + (int64_t)n0 * a.ld_w, a.ld_w, a.vocab - n0, a.dim};
-        L.next(O);
+        return vg_rows(a.weight + (int64_t)n0 * a.ld_w, a.ld_w, a.vocab - n0, a.dim);
       },
-      [&](int, char* w) {
-        Words<C>::bring(a, A.vt * C::BN, (int64_t)A.rb * C::BM, false, w);
-        A.next(O);
+      [&](int i, char* w) {
+        Walk A = M;
+        if (i >= 0) A.next(O);
+        Words<C>::bring(a, A.vt * C::BN, (int64_t)M.rb * C::BM, false, w);
       },
-      [&](int, f32x4 (&acc)[C::MI][C::NI], char* w) { Words<C>::start(a, M.vt * C::BN, wn, lq, w, acc); },
-      [&](int, f32x4 (&acc)[C::MI][C::NI], char* w) {
+      [&](int, f32x4 (&acc)[C::MI][C::NI], char* w) { Words<C>::start(a, M.vt * C::BN, wn, w, acc); },
+      [&](int, f32x4 (&acc)[C::MI][C::NI], char* slot) {
+        const int lane = vg_lane(), l16 = lane & 15, lq = lane >> 4;
+        const char* w = slot + C::O_WORDS;
         const int rb = M.rb, tn = M.vt;
         const int n0 = tn * C::BN + wn * 16 * C::NI + lq * 4;      // this lane's columns: n0 + j * 16 + e
 #pragma unroll
@@ -430,9 +440,7 @@ __device__ __forceinline__ void lse_body(const LossArgs& a, char* smem) {
         M.next(O);
         if (more) return;
         // the last tile of this row block here: the four lanes of a row, then the waves that share it
-        float2* red = reinterpret_cast<float2*>(smem + C::O_SLAB);      // [WN][BM]
-        static_assert(C::WN * C::BM * 8 <= C::WAVES * C::SLAB, "the joint of the waves fits the slabs");
-        __syncthreads();
+        float2* red = reinterpret_cast<float2*>(slot + C::O_RED);      // [WN][BM]
 #pragma unroll
         for (int q = 0; q < C::MI; ++q) {
           float m = -nref[q], s = sm[q];
@@ -545,31 +553,33 @@ __global__ __launch_bounds__(1024) void reduce_kernel(LossArgs a) {
 // ------------------------------------------------------------------------------------------------------------------------------------
 template <typename C>
 __device__ __forceinline__ void dlogits_body(const LossArgs& a, char* smem) {
-  const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
   const Order O(*a.count, a.piece, C::BM, C::BN, gridDim.x, blockIdx.x & 7);
-  Walk L(O, blockIdx.x >> 3), A = L, M = L;      // operands, words, sums
+  Walk L(O, blockIdx.x >> 3), M = L;      // the operands, the results
   const int tiles = M.left(O);
   if (tiles == 0) return;
   const float cs = a.inv_t * LOG2E;
   const bool label = !a.topk;
-  char* slab = smem + C::O_SLAB + wave * C::SLAB;
-  vg_run<C, false, false, true>(
+  vg_run<C, false, false, true, true, true>(
       tiles, smem,
       [&](int, int& k0, int& k1) { k0 = 0; k1 = a.hp / VG_K; },
-      [&](int, VgOperand& X, VgOperand& W) {
+      [&](int) { return vg_rows(a.hc + (int64_t)L.rb * C::BM * a.hp, a.hp, C::BM, a.hp); },      // of the tile whose weights were asked for before
+      [&](int i) {
+        if (i > 0) L.next(O);
         const int n0 = a.v0 + L.vt * C::BN;
-        X = VgOperand{a.hc + (int64_t)L.rb * C::BM * a.hp, a.hp, C::BM, a.hp};
-        W = VgOperand{a.weight + (int64_t)min(n0, a.vocab - 1) * a.ld_w, a.ld_w, max(1, a.vocab - n0), a.dim};
-        L.next(O);
+        return vg_rows(a.weight + (int64_t)min(n0, a.vocab - 1) * a.ld_w, a.ld_w, max(1, a.vocab - n0), a.dim);
       },
-      [&](int, char* w) {
-        Words<C>::bring(a, a.v0 + A.vt * C::BN, (int64_t)A.rb * C::BM, true, w);
-        A.next(O);
+      [&](int i, char* w) {
+        Walk A = M;
+        if (i >= 0) A.next(O);
+        Words<C>::bring(a, a.v0 + A.vt * C::BN, (int64_t)M.rb * C::BM, true, w);
       },
-      [&](int, f32x4 (&acc)[C::MI][C::NI], char* w) { Words<C>::start(a, a.v0 + M.vt * C::BN, wn, lq, w, acc); },
-      [&](int, f32x4 (&acc)[C::MI][C::NI], char* w) {
+      [&](int, f32x4 (&acc)[C::MI][C::NI], char* w) { Words<C>::start(a, a.v0 + M.vt * C::BN, wn, w, acc); },
+      [&](int, f32x4 (&acc)[C::MI][C::NI], char* slot) {
+        const int lane = vg_lane(), l16 = lane & 15, lq = lane >> 4;
+        const char* w = slot + C::O_WORDS;
+        char* slab = slot + wave * C::SLAB;
         const int tm = M.rb, tn = M.vt;
         M.next(O);
         const int64_t m0 = (int64_t)tm * C::BM + wm * 16 * C::MI;
@@ -607,7 +617,8 @@ __device__ __forceinline__ void dlogits_body(const LossArgs& a, char* smem) {
             vg_slab_put<C>(slab, l16, lq, j, p[j]);
           }
           CACO_WAVE_LDS_SYNC();
-          vg_slab_rows<C>(slab, lane, [&](int r, int ch, bf16x8 v) { *reinterpret_cast<bf16x8*>(a.dl + (m0 + q * 16 + r) * a.piece + c0 + ch * 8) = v; });
+          bf16_t* d = dl_at(a, m0 + q * 16, c0);      // 16 rows and the wave's columns lie in one block
+          vg_slab_rows<C>(slab, lane, [&](int r, int ch, bf16x8 v) { *reinterpret_cast<bf16x8*>(d + r * 256 + ch * 8) = v; });
           CACO_WAVE_LDS_SYNC();
         }
         if (a.db) {
@@ -645,7 +656,7 @@ __global__ __launch_bounds__(256) void targets2_kernel(LossArgs a) {
   const int idx = a.tgt_idx[t], v = idx - a.v0;
   const float g = a.g[c], q = a.tgt_q[t];
   if (idx < 0 || v < 0 || v >= a.piece || g == 0.f || q == 0.f) return;
-  a.dl[c * a.piece + v] = (bf16_t)(g * __builtin_amdgcn_exp2f(a.tgt_z[t] - a.lse2[c]) - g * q);
+  *dl_at(a, c, v) = (bf16_t)(g * __builtin_amdgcn_exp2f(a.tgt_z[t] - a.lse2[c]) - g * q);
   if (!a.db) return;
   const float x = ldexpf(g * q, 38 - fixed_exponent(a));
   if (fabsf(x) <= 0x1p38f) atomicAdd(a.db64 + idx, (unsigned long long)(long long)rintf(x));
@@ -721,25 +732,28 @@ struct Share {
 
 __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
   typedef Big C;
-  const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
   const int n = *a.count;
   const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
   const Share S(a, n, gridDim.x, xcd);
-  char* slab = smem + C::O_SLAB + wave * C::SLAB;
   // d weight: both operands with the token slowest
   if (slot < S.wcnt)
-    vg_run<C, true, true, false>(
+    vg_run<C, true, true, false, false, false>(
         (S.wcnt - slot + S.slots - 1) / S.slots, smem,
         [&](int, int& k0, int& k1) { k0 = 0; k1 = S.nkw; },
-        [&](int i, VgOperand& X, VgOperand& W) {
-          const int t = S.wbase + slot + i * S.slots, tn = t % S.cb, tm = t / S.cb;
-          X = VgOperand{a.dl + tm * C::BM, a.piece, C::BM, (int64_t)S.nkw * VG_K};
-          W = VgOperand{a.hc + tn * C::BN, a.hp, a.hp - tn * C::BN, (int64_t)S.nkw * VG_K};
+        [&](int i) {
+          const int tm = (S.wbase + slot + i * S.slots) / S.cb;
+          return VgOperand{a.dl + (int64_t)tm * 65536, 256, C::BM, (int64_t)S.nkw * VG_K, VG_K * 256, (int64_t)a.piece * 256};
         },
-        VgNoAux{}, VgZero{},
-        [&](int i, f32x4 (&acc)[C::MI][C::NI], char*) {
+        [&](int i) {
+          const int c = (S.wbase + slot + i * S.slots) % S.cb * C::BN;
+          return vg_cols(a.hc + c, a.hp, a.hp - c, (int64_t)S.nkw * VG_K);
+        },
+        VgNoWords{}, VgZero{},
+        [&](int i, f32x4 (&acc)[C::MI][C::NI], char* free_slot) {
+          const int lane = vg_lane(), l16 = lane & 15, lq = lane >> 4;
+          char* slab = free_slot + wave * C::SLAB;
           const int t = S.wbase + slot + i * S.slots, tn = t % S.cb, tm = t / S.cb;
           const int v0 = a.v0 + tm * C::BM + wm * 16 * C::MI, c0 = tn * C::BN + wn * 16 * C::NI;
 #pragma unroll
@@ -760,21 +774,22 @@ __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
   if (parts == 0) return;
   const bool first_piece = a.v0 == 0;
   auto out_tile = [&](int i) { return i < S.whole ? S.t0 + slot + i * S.slots : S.t0 + S.whole * S.slots + l0 + i - S.whole; };
-  vg_run<C, false, true, false>(
+  vg_run<C, false, true, false, false, false>(
       parts, smem,
       [&](int i, int& k0, int& k1) {
         const int at = i < S.whole ? 0 : (l0 + i - S.whole) * S.nkx;      // the tile's first K-tile in the list
         k0 = S.k0 + (i < S.whole ? 0 : max(0, f0 - at));
         k1 = S.k0 + (i < S.whole ? S.nkx : min(S.nkx, f1 - at));
       },
-      [&](int i, VgOperand& X, VgOperand& W) {
-        const int o = out_tile(i), cb = o % S.cb, rb = o / S.cb;
-        X = VgOperand{a.dl + (int64_t)rb * C::BM * a.piece, a.piece, C::BM, a.piece};
-        W = VgOperand{a.weight + (int64_t)a.v0 * a.ld_w + cb * C::BN, a.ld_w, a.dim - cb * C::BN, a.vocab - a.v0};
+      [&](int i) { return VgOperand{a.dl + (int64_t)(out_tile(i) / S.cb) * C::BM * a.piece, 256, C::BM, a.piece, VG_K, 65536}; },
+      [&](int i) {
+        const int c = out_tile(i) % S.cb * C::BN;
+        return vg_cols(a.weight + (int64_t)a.v0 * a.ld_w + c, a.ld_w, a.dim - c, a.vocab - a.v0);
       },
-      VgNoAux{}, VgZero{},
+      VgNoWords{}, VgZero{},
       [&](int i, f32x4 (&acc)[C::MI][C::NI], char*) {
         const int o = out_tile(i), rb = o / S.cb;
+        const int lane = vg_lane(), l16 = lane & 15, lq = lane >> 4;
         const int64_t place = i < S.whole ? S.slab_whole(o) : S.slab_list(xcd, l0 + i - S.whole, slot);
         float* d = a.slab + place * C::BM * C::BN + (wm * 16 * C::MI + l16) * C::BN + wn * 16 * C::NI + lq * 4;
 #pragma unroll
@@ -920,16 +935,16 @@ int run_loss(LossArgs& a, const Plan& P, int what, int cus, hipStream_t st) {
   CACO_TRY_RC(launch("loss gather", gather_kernel, pad4, 256, 0, st, a, (int)bwd, (int)!fwd));
   if (a.topk) CACO_TRY_RC(launch("loss target logits", target_logits_kernel, pad4, 256, 0, st, a));
   if (fwd) {
-    CACO_TRY_RC(launch("loss lse", lse_kernel<C>, dim3(wgs), C::THREADS, C::SMEM, st, a));
+    CACO_TRY_RC(launch("loss lse", lse_kernel<C>, dim3(wgs), C::THREADS, C::SMEM_WFAR, st, a));
     if (a.rows) CACO_TRY_RC(launch("loss finish", finish_kernel, rows4, 256, 0, st, a, (int)C::BM, (int)C::BN, wgs));
     if (a.loss) CACO_TRY_RC(launch("loss reduce", reduce_kernel, dim3(1), 1024, 0, st, a));
   }
   if (!bwd) return CACO_OK;
   for (; a.v0 < a.vocab; a.v0 += a.piece) {
-    CACO_TRY_RC(launch("loss dlogits", dlogits_kernel<C>, dim3(wgs), C::THREADS, C::SMEM, st, a));
+    CACO_TRY_RC(launch("loss dlogits", dlogits_kernel<C>, dim3(wgs), C::THREADS, C::SMEM_WFAR, st, a));
     if (a.topk) CACO_TRY_RC(launch("loss targets2", targets2_kernel, dim3((unsigned)(P.npad * a.kp / 256)), 256, 0, st, a));
     if (a.db) CACO_TRY_RC(launch("loss dbias", dbias_kernel, dim3((a.piece + 255) / 256), 256, 0, st, a, (int)C::BM, (int)C::WM));
-    if (a.dh || a.dw) CACO_TRY_RC(launch("loss grads", grads_kernel, dim3(cus), Big::THREADS, Big::SMEM, st, a));
+    if (a.dh || a.dw) CACO_TRY_RC(launch("loss grads", grads_kernel, dim3(cus), Big::THREADS, Big::SMEM_XFAR, st, a));
   }
   if (a.dh && a.rows) CACO_TRY_RC(launch("loss dhidden join", dh_join_kernel, rows4, 256, 0, st, a, cus));
   return CACO_OK;
@@ -1006,7 +1021,7 @@ int linear_loss(const LinearLoss& c, hipStream_t st) {
   a.wmax = (float*)(a.count + 1); a.db64 = (unsigned long long*)(w + P.o_db64);
   a.piece = (int)piece;
   int num_cu = 0;
-  CACO_TRY_RC(prepare_launch(reinterpret_cast<const void*>(&lse_kernel<Big>), Big::SMEM, &num_cu));
+  CACO_TRY_RC(prepare_launch(reinterpret_cast<const void*>(&lse_kernel<Big>), Big::SMEM_WFAR, &num_cu));
   // a power of two of workgroups per XCD, 8 at least (Order)
   int cus = 64;
   while (cus * 2 <= num_cu && cus < MAX_CU) cus *= 2;
