@@ -49,7 +49,7 @@ struct LossArgs {
   const void* teacher_idx; int64_t ld_i; int idx64;
   int topk, kp;                      // entries per row; kp = next power of two, the pitch of the target lists
   float inv_t, temperature;
-  int64_t rows; int vocab, dim, hp;  // hp = dim rounded up to the K-tile
+  int64_t rows, npad; int vocab, dim, hp;      // npad, hp: rows rounded up to 256, dim to the K-tile
   int reduction;
   const float* row_weight;
   const float* grad_scale;
@@ -63,6 +63,7 @@ struct LossArgs {
   int *tgt_idx0; float *tgt_q0;      // targets in the caller's order [rows, kp] (distillation)
   int *tgt_idx; float *tgt_q;        // targets of the compact rows [npad, kp]
   bf16_t* hc;                        // [npad, hp]
+  bf16_t* hct;                       // [hp, npad]: its transpose, for d weight
   float2* part;                      // (max, sum) of log2-logits, [group of row blocks][workgroup][rows of a block]
   float* zt;                         // cross entropy: the label's log2-logit; distillation: sum_k q_k (z_k / T - log q_k), log2 units
   float* tgt_z;                      // distillation: the entries' log2-logits [npad, kp]
@@ -227,6 +228,28 @@ __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, i
   }
 }
 
+// hct <- hc, 64 x 64 at a time through the LDS; columns of rows past the last block of 256 that counts are never read
+__global__ __launch_bounds__(256) void transpose_kernel(LossArgs a) {
+  __shared__ bf16_t s_t[64][72];
+  const int64_t c0 = (int64_t)blockIdx.x * 64;
+  const int h0 = blockIdx.y * 64, t = threadIdx.x;
+  if (c0 >= ((int64_t)*a.count + 255) / 256 * 256) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = i * 32 + t / 8, k = t % 8 * 8;
+    *reinterpret_cast<bf16x8*>(&s_t[r][k]) = *reinterpret_cast<const bf16x8*>(a.hc + (c0 + r) * a.hp + h0 + k);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int h = i * 32 + t / 8, r = t % 8 * 8;
+    bf16x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = s_t[r + e][h];
+    *reinterpret_cast<bf16x8*>(a.hct + (h0 + h) * a.npad + c0 + r) = v;
+  }
+}
+
 // (distillation) sum_k q_k (log q_k - z_k / T) of a compact row: 16 lanes per entry, the entries' rows of weight gathered.
 // Also in log2 units, so that `finish` treats both losses alike.
 __global__ __launch_bounds__(256) void target_logits_kernel(LossArgs a) {
@@ -377,11 +400,11 @@ __device__ __forceinline__ void lse_body(const LossArgs& a, char* smem) {
   vg_run<C, false, false, true, true, true>(
       tiles, smem,
       [&](int, int& k0, int& k1) { k0 = 0; k1 = a.hp / VG_K; },
-      [&](int) { return vg_rows(a.hc + (int64_t)L.rb * C::BM * a.hp, a.hp, C::BM, a.hp); },      // of the tile whose weights were asked for before
+      [&](int) { return VgOperand{a.hc + (int64_t)L.rb * C::BM * a.hp, a.hp, C::BM, a.hp, 0}; },      // of the tile whose weights were asked for before
       [&](int i) {
         if (i > 0) L.next(O);
         const int n0 = L.vt * C::BN;
-        return vg_rows(a.weight + (int64_t)n0 * a.ld_w, a.ld_w, a.vocab - n0, a.dim);
+        return VgOperand{a.weight + (int64_t)n0 * a.ld_w, a.ld_w, a.vocab - n0, a.dim, 0};
       },
       [&](int i, char* w) {
         Walk A = M;
@@ -564,11 +587,11 @@ __device__ __forceinline__ void dlogits_body(const LossArgs& a, char* smem) {
   vg_run<C, false, false, true, true, true>(
       tiles, smem,
       [&](int, int& k0, int& k1) { k0 = 0; k1 = a.hp / VG_K; },
-      [&](int) { return vg_rows(a.hc + (int64_t)L.rb * C::BM * a.hp, a.hp, C::BM, a.hp); },      // of the tile whose weights were asked for before
+      [&](int) { return VgOperand{a.hc + (int64_t)L.rb * C::BM * a.hp, a.hp, C::BM, a.hp, 0}; },      // of the tile whose weights were asked for before
       [&](int i) {
         if (i > 0) L.next(O);
         const int n0 = a.v0 + L.vt * C::BN;
-        return vg_rows(a.weight + (int64_t)min(n0, a.vocab - 1) * a.ld_w, a.ld_w, max(1, a.vocab - n0), a.dim);
+        return VgOperand{a.weight + (int64_t)min(n0, a.vocab - 1) * a.ld_w, a.ld_w, max(1, a.vocab - n0), a.dim, 0};
       },
       [&](int i, char* w) {
         Walk A = M;
@@ -614,12 +637,14 @@ __device__ __forceinline__ void dlogits_body(const LossArgs& a, char* smem) {
 #pragma unroll
           for (int j = 0; j < C::NI; ++j) {
             col[j] += p[j];
+            vg_here(col[j]);
             vg_slab_put<C>(slab, l16, lq, j, p[j]);
           }
           CACO_WAVE_LDS_SYNC();
           bf16_t* d = dl_at(a, m0 + q * 16, c0);      // 16 rows and the wave's columns lie in one block
           vg_slab_rows<C>(slab, lane, [&](int r, int ch, bf16x8 v) { *reinterpret_cast<bf16x8*>(d + r * 256 + ch * 8) = v; });
           CACO_WAVE_LDS_SYNC();
+          __builtin_amdgcn_sched_barrier(0);      // one row block's registers at a time
         }
         if (a.db) {
 #pragma unroll
@@ -737,18 +762,18 @@ __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
   const int n = *a.count;
   const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
   const Share S(a, n, gridDim.x, xcd);
-  // d weight: both operands with the token slowest
+  // d weight: d logits with the token slowest, the transposed hidden states with the token fastest
   if (slot < S.wcnt)
-    vg_run<C, true, true, false, false, false>(
+    vg_run<C, true, false, false, false, false>(
         (S.wcnt - slot + S.slots - 1) / S.slots, smem,
         [&](int, int& k0, int& k1) { k0 = 0; k1 = S.nkw; },
         [&](int i) {
           const int tm = (S.wbase + slot + i * S.slots) / S.cb;
-          return VgOperand{a.dl + (int64_t)tm * 65536, 256, C::BM, (int64_t)S.nkw * VG_K, VG_K * 256, (int64_t)a.piece * 256};
+          return VgOperand{a.dl + (int64_t)tm * 65536, 256, C::BM, S.nkw * VG_K, (int64_t)a.piece * 256};
         },
         [&](int i) {
           const int c = (S.wbase + slot + i * S.slots) % S.cb * C::BN;
-          return vg_cols(a.hc + c, a.hp, a.hp - c, (int64_t)S.nkw * VG_K);
+          return VgOperand{a.hct + c * a.npad, a.npad, a.hp - c, S.nkw * VG_K, 0};
         },
         VgNoWords{}, VgZero{},
         [&](int i, f32x4 (&acc)[C::MI][C::NI], char* free_slot) {
@@ -781,10 +806,10 @@ __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
         k0 = S.k0 + (i < S.whole ? 0 : max(0, f0 - at));
         k1 = S.k0 + (i < S.whole ? S.nkx : min(S.nkx, f1 - at));
       },
-      [&](int i) { return VgOperand{a.dl + (int64_t)(out_tile(i) / S.cb) * C::BM * a.piece, 256, C::BM, a.piece, VG_K, 65536}; },
+      [&](int i) { return VgOperand{a.dl + (int64_t)(out_tile(i) / S.cb) * C::BM * a.piece, 256, C::BM, a.piece, 65536}; },
       [&](int i) {
         const int c = out_tile(i) % S.cb * C::BN;
-        return vg_cols(a.weight + (int64_t)a.v0 * a.ld_w + c, a.ld_w, a.dim - c, a.vocab - a.v0);
+        return VgOperand{a.weight + (int64_t)a.v0 * a.ld_w + c, a.ld_w, a.dim - c, a.vocab - a.v0, 0};
       },
       VgNoWords{}, VgZero{},
       [&](int i, f32x4 (&acc)[C::MI][C::NI], char*) {
@@ -810,51 +835,49 @@ __global__ __launch_bounds__(Big::THREADS) __attribute__((amdgpu_waves_per_eu(2,
   grads_body(a, smem);
 }
 
-// rows of d hidden in the caller's order, 4 to a workgroup: the parts added in order and rounded once; zeros for rows that do not count
+// d hidden's parts added in order and rounded once: 16 compact rows x 256 of dim to a workgroup.  It also writes zeros to those of the
+// caller's rows with the same numbers that do not count.
 __global__ __launch_bounds__(256) void dh_join_kernel(LossArgs a, int wgs) {
-  __shared__ int s_first[8][MAX_CU / 8 + 1];
-  const int slots = wgs >> 3, n = *a.count;
-  for (int w = threadIdx.x; w < 8 * (slots + 1); w += 256) {
-    const int x = w / (slots + 1), s = w % (slots + 1);
-    s_first[x][s] = Share(a, n, wgs, x).first(s);
+  __shared__ int64_t s_place[8][MAX_CU / 8 + 1];
+  __shared__ int s_parts[8];
+  const int n = *a.count, t = threadIdx.x;
+  const int64_t c0 = (int64_t)blockIdx.x * 16;
+  const int x = blockIdx.y * 256 + t % 32 * 8;
+  for (int64_t r = c0 + t / 32; r < c0 + 16; r += 8)
+    if (r < a.rows && x < a.dim && a.inv[r] < 0) *reinterpret_cast<bf16x8*>(a.dh + r * a.ld_dh + x) = bf16x8{};
+  if (c0 >= n) return;
+  // where the parts of this output tile are: one thread per XCD
+  if (t < 8) {
+    const Share S(a, n, wgs, t);
+    const int o = (int)(c0 / 256) * S.cb + blockIdx.y, i = o - S.t0 - S.whole * S.slots;      // the tile's place in the list
+    int parts = 0;
+    if (o >= S.t0 && i < S.rest) {
+      if (i < 0) s_place[t][parts++] = S.slab_whole(o);
+      else
+        for (int s = 0; s < S.slots && S.first(s) < (i + 1) * S.nkx; ++s)
+          if (S.first(s + 1) > i * S.nkx && S.first(s + 1) > S.first(s)) s_place[t][parts++] = S.slab_list(t, i, s);
+    }
+    s_parts[t] = parts;
   }
   __syncthreads();
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= a.rows) return;
-  const int c = a.inv[row];
-  for (int x = lane * 8; x < a.dim; x += 512) {
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (c >= 0) {
-      const Share S0(a, n, wgs, 0);
-      const int o = c / 256 * S0.cb + x / 256, groups = 8 / S0.ks;
-      int grp = 0;
-      while (grp + 1 < groups && (int)((int64_t)(grp + 1) * S0.tiles / groups) <= o) ++grp;
-      for (int slice = 0; slice < S0.ks; ++slice) {
-        const int xcd = grp * S0.ks + slice;
-        const Share S(a, n, wgs, xcd);
-        auto add = [&](int64_t place) {
-          const float* p = a.slab + place * 65536 + c % 256 * 256 + x % 256;
-          const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
+  if (x >= a.dim) return;
+  f32x4 v[2][2] = {};
+  const int r0 = (int)(c0 % 256) + t / 32;
+  for (int xcd = 0; xcd < 8; ++xcd)
+    for (int k = 0; k < s_parts[xcd]; ++k) {
+      const float* p = a.slab + s_place[xcd][k] * 65536 + r0 * 256 + t % 32 * 8;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { v[e] += lo[e]; v[e + 4] += hi[e]; }
-        };
-        const int i = o - S.t0 - S.whole * slots;      // its place in the list
-        if (i < 0) {
-          add(S.slab_whole(o));
-          continue;
-        }
-        int s = 0;                                       // the last workgroup that begins no later than the tile, then its neighbours
-        for (int b = MAX_CU / 8; b > 0; b >>= 1)
-          if (s + b < slots && s_first[xcd][s + b] <= i * S.nkx) s += b;
-        for (; s < slots && s_first[xcd][s] < (i + 1) * S.nkx; ++s)
-          if (s_first[xcd][s] < s_first[xcd][s + 1]) add(S.slab_list(xcd, i, s));
-      }
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) v[i][h] += *reinterpret_cast<const f32x4*>(p + i * 8 * 256 + h * 4);
     }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t c = c0 + t / 32 + i * 8;
     bf16x8 o8;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o8[e] = (bf16_t)v[e];
-    *reinterpret_cast<bf16x8*>(a.dh + row * a.ld_dh + x) = o8;
+    for (int e = 0; e < 8; ++e) o8[e] = (bf16_t)v[i][e / 4][e % 4];
+    if (c < n) *reinterpret_cast<bf16x8*>(a.dh + (int64_t)a.rowmap[c] * a.ld_dh + x) = o8;
   }
 }
 
@@ -869,7 +892,7 @@ struct Plan {
   int hp, kp;
   int64_t piece;
   bool small;
-  int64_t o_count, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_part, o_zt, o_lse2, o_g, o_db64, o_dl, o_slab, o_dbp;
+  int64_t o_count, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_hct, o_part, o_zt, o_lse2, o_g, o_db64, o_dl, o_slab, o_dbp;
   int64_t take(int64_t n) {
     const int64_t at = bytes;
     bytes += up(n, 256);
@@ -897,9 +920,10 @@ struct Plan {
     o_lse2 = take(npad * 4);
     o_g = take(npad * 4);
     piece = piece_cols;
-    o_db64 = o_dl = o_slab = o_dbp = 0;
+    o_hct = o_db64 = o_dl = o_slab = o_dbp = 0;
     if (piece) {
       if (topk) o_db64 = take((int64_t)vocab * 8);
+      o_hct = take((int64_t)hp * npad * 2);
       o_dl = take(npad * piece * 2);
       o_slab = take(Share::slabs(npad / 256 * ((dim + 255) / 256), MAX_CU / 8) * 65536 * 4);
       o_dbp = take(npad / bm * (small ? Small::WM : Big::WM) * piece * 4);
@@ -940,13 +964,14 @@ int run_loss(LossArgs& a, const Plan& P, int what, int cus, hipStream_t st) {
     if (a.loss) CACO_TRY_RC(launch("loss reduce", reduce_kernel, dim3(1), 1024, 0, st, a));
   }
   if (!bwd) return CACO_OK;
+  if (a.dw) CACO_TRY_RC(launch("loss transpose", transpose_kernel, dim3((unsigned)(P.npad / 64), a.hp / 64), 256, 0, st, a));
   for (; a.v0 < a.vocab; a.v0 += a.piece) {
     CACO_TRY_RC(launch("loss dlogits", dlogits_kernel<C>, dim3(wgs), C::THREADS, C::SMEM_WFAR, st, a));
     if (a.topk) CACO_TRY_RC(launch("loss targets2", targets2_kernel, dim3((unsigned)(P.npad * a.kp / 256)), 256, 0, st, a));
     if (a.db) CACO_TRY_RC(launch("loss dbias", dbias_kernel, dim3((a.piece + 255) / 256), 256, 0, st, a, (int)C::BM, (int)C::WM));
     if (a.dh || a.dw) CACO_TRY_RC(launch("loss grads", grads_kernel, dim3(cus), Big::THREADS, Big::SMEM_XFAR, st, a));
   }
-  if (a.dh && a.rows) CACO_TRY_RC(launch("loss dhidden join", dh_join_kernel, rows4, 256, 0, st, a, cus));
+  if (a.dh && a.rows) CACO_TRY_RC(launch("loss dhidden join", dh_join_kernel, dim3((unsigned)((a.rows + 15) / 16), (a.dim + 255) / 256), 256, 0, st, a, cus));
   return CACO_OK;
 }
 
@@ -1009,14 +1034,14 @@ int linear_loss(const LinearLoss& c, hipStream_t st) {
   a.topk = c.topk; a.kp = P.kp;
   a.temperature = c.topk ? c.temperature : 1.f;
   a.inv_t = 1.f / a.temperature;
-  a.rows = c.rows; a.vocab = c.vocab; a.dim = c.dim; a.hp = P.hp;
+  a.rows = c.rows; a.npad = P.npad; a.vocab = c.vocab; a.dim = c.dim; a.hp = P.hp;
   a.reduction = c.reduction; a.row_weight = c.row_weight; a.grad_scale = c.grad_scale;
   a.row_loss = c.row_loss; a.lse = c.lse; a.loss = c.loss;
   a.dh = bwd ? c.d_hidden : nullptr; a.ld_dh = c.ld_dh; a.dw = bwd ? c.d_weight : nullptr; a.ld_dw = c.ld_dw; a.db = bwd ? c.d_bias : nullptr;
   char* w = reinterpret_cast<char*>(c.ws);
   a.count = (int*)(w + P.o_count); a.rowmap = (int*)(w + P.o_rowmap); a.inv = (int*)(w + P.o_inv);
   a.tgt_idx0 = (int*)(w + P.o_ti0); a.tgt_q0 = (float*)(w + P.o_tq0); a.tgt_idx = (int*)(w + P.o_ti); a.tgt_q = (float*)(w + P.o_tq);
-  a.hc = (bf16_t*)(w + P.o_hc); a.part = (float2*)(w + P.o_part); a.zt = (float*)(w + P.o_zt); a.tgt_z = (float*)(w + P.o_tz); a.lse2 = (float*)(w + P.o_lse2); a.g = (float*)(w + P.o_g);
+  a.hc = (bf16_t*)(w + P.o_hc); a.hct = (bf16_t*)(w + P.o_hct); a.part = (float2*)(w + P.o_part); a.zt = (float*)(w + P.o_zt); a.tgt_z = (float*)(w + P.o_tz); a.lse2 = (float*)(w + P.o_lse2); a.g = (float*)(w + P.o_g);
   a.dl = (bf16_t*)(w + P.o_dl); a.slab = (float*)(w + P.o_slab); a.dbp = (float*)(w + P.o_dbp);
   a.wmax = (float*)(a.count + 1); a.db64 = (unsigned long long*)(w + P.o_db64);
   a.piece = (int)piece;
