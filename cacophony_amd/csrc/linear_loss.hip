@@ -35,6 +35,9 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int MAX_WG = 512;          // most workgroups of a persistent launch (two per CU)
 constexpr int MAX_CU = 256;
+// From this many rows on d hidden reads transposed weights.  Transposing costs 4 bytes of traffic per weight, whatever the rows; it saves 0.65 us
+// per K-tile and workgroup, which pays from about 1300 rows on (768 x 50265: 35 us against 130 us at 5489 rows, 30 at 1187).
+constexpr int WT_ROWS = 2048;
 
 typedef VgTile<8, 4, 2, 4> Big;      // 256 x 256, one workgroup per CU
 typedef VgTile<4, 2, 1, 4> Small;    // 64 x 128, two per CU: 64 tokens or fewer, where a call reads the weights and does little else
@@ -70,9 +73,12 @@ struct LossArgs {
   float *lse2, *g;                   // compact: lse in log2 units, gradient scale of the row
   float* wmax;                       // largest |row_weight| of the rows that count
   unsigned long long* db64;          // distillation: sum of the targets' weights per word, fixed point in units of 2^(e - 38), |g| < 2^e
-  // d logits of the piece in blocks of 256 rows x 256 columns, [row block][column block][256][256]: a K-tile of either gradient is then 32 KiB
-  // next to one another or 256 rows 512 bytes apart, instead of rows a whole piece apart (100 KB at 50265 words)
-  bf16_t* dl;
+  // d logits of the piece in blocks of 256 rows x 256 columns, [row block][column block][256][256], once with the columns next to one another
+  // (d hidden sums over them) and once with the rows (d weight): both products then read fragments of 16 bytes.  (One copy and
+  // transposing reads in one of the products: 2.2 us per K-tile of it instead of 1.6; those reads and the loads into LDS get in each
+  // other's way, either alone is as fast.)
+  bf16_t *dl, *dlt;
+  bf16_t* wt;                        // the piece's weights transposed [dim, piece], zeros past the vocabulary; or null
   float* slab;                       // d hidden's partial sums [output tile + workgroup][256][256]
   float* dbp;                        // [row halves, piece]
   int piece, v0;                     // columns of the piece, its first column
@@ -138,10 +144,8 @@ __global__ __launch_bounds__(256) void targets_kernel(LossArgs a) {
   if (lane == 0) a.inv[row] = some;                        // for `compact`
 }
 
-// a row of one 256 x 256 block of d logits
-__device__ __forceinline__ bf16_t* dl_at(const LossArgs& a, int64_t row, int col) {
-  return a.dl + (((row >> 8) * (a.piece >> 8) + (col >> 8)) * 256 + (row & 255)) * 256 + (col & 255);
-}
+// the 256 x 256 block of d logits that holds (row, col)
+__device__ __forceinline__ int64_t dl_block(const LossArgs& a, int64_t row, int col) { return ((row >> 8) * (a.piece >> 8) + (col >> 8)) * 65536; }
 
 // does row r count?
 __device__ __forceinline__ bool row_counts(const LossArgs& a, int64_t r) {
@@ -152,43 +156,41 @@ __device__ __forceinline__ bool row_counts(const LossArgs& a, int64_t r) {
   return a.inv[r] != 0;
 }
 
-// One workgroup: every thread counts a run of consecutive rows, a scan over the threads gives each run its first place.
+// One workgroup: every wave counts a run of consecutive rows, 64 at a time; a scan over the waves gives each run its first place.
 // Also the largest |row_weight| of the rows that count.
 __global__ __launch_bounds__(1024) void compact_kernel(LossArgs a) {
-  __shared__ int s_wave[16];
+  __shared__ int s_n[16];
   __shared__ float s_max[16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t per = (a.rows + 1023) / 1024;
-  const int64_t r0 = min(a.rows, tid * per), r1 = min(a.rows, r0 + per);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t per = (a.rows + 1023) / 1024 * 64;
+  const int64_t r0 = min(a.rows, wave * per), r1 = min(a.rows, r0 + per);
   int n = 0;
-  for (int64_t r = r0; r < r1; ++r) n += row_counts(a, r);
-  int incl = n;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int v = __shfl(incl, max(lane - o, 0), 64);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 63) s_wave[wave] = incl;
+  for (int64_t r = r0; r < r1; r += 64) n += __builtin_popcountll(__ballot(r + lane < r1 && row_counts(a, min(r + lane, r1 - 1))));
+  if (lane == 0) s_n[wave] = n;
   __syncthreads();
-  int at = incl - n;
+  int at = 0;
+  for (int w = 0; w < wave; ++w) at += s_n[w];
   float wmax = a.row_weight ? 0.f : 1.f;
-  for (int w = 0; w < wave; ++w) at += s_wave[w];
-  for (int64_t r = r0; r < r1; ++r) {
-    const bool c = row_counts(a, r);      // this thread's own rows: read before they are overwritten
-    a.inv[r] = c ? at : -1;
+  for (int64_t r = r0; r < r1; r += 64) {
+    const int64_t row = r + lane;
+    const bool c = row < r1 && row_counts(a, min(row, r1 - 1));      // this wave's own rows: read before they are overwritten
+    const unsigned long long mask = __ballot(c);
+    const int place = at + __builtin_popcountll(mask & ((1ull << lane) - 1));
+    if (row < r1) a.inv[row] = c ? place : -1;
     if (c) {
-      a.rowmap[at++] = (int)r;
-      if (a.row_weight) wmax = fmaxf(wmax, fabsf(a.row_weight[r]));
+      a.rowmap[place] = (int)row;
+      if (a.row_weight) wmax = fmaxf(wmax, fabsf(a.row_weight[row]));
     }
+    at += __builtin_popcountll(mask);
   }
   wmax = wave_max(wmax);
   if (lane == 0) s_max[wave] = wmax;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < 16; ++w) wmax = fmaxf(wmax, s_max[w]);
+  if (threadIdx.x == 1023) {
+    for (int w = 0; w < 16; ++w) wmax = fmaxf(wmax, s_max[w]);
     *a.wmax = wmax;
+    *a.count = at;
   }
-  if (tid == 1023) *a.count = at;
 }
 
 // T from the logits' scale and the loss's T^2, the row's weight, the incoming gradient, the mean
@@ -228,16 +230,18 @@ __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, i
   }
 }
 
-// hct <- hc, 64 x 64 at a time through the LDS; columns of rows past the last block of 256 that counts are never read
-__global__ __launch_bounds__(256) void transpose_kernel(LossArgs a) {
+// dst [cols, ld_d] <- src [rows, cols] (ld_s), 64 x 64 at a time through the LDS; rows past the end become zeros, columns past the end (8 of them
+// exist or none) are not written.  `blocks`: if given, only the rows of the first *blocks / 256 (rounded up) blocks of 256 are looked at.
+__global__ __launch_bounds__(256) void transpose_kernel(const bf16_t* src, int64_t ld_s, int64_t rows, int cols, bf16_t* dst, int64_t ld_d, const int* blocks) {
   __shared__ bf16_t s_t[64][72];
   const int64_t c0 = (int64_t)blockIdx.x * 64;
   const int h0 = blockIdx.y * 64, t = threadIdx.x;
-  if (c0 >= ((int64_t)*a.count + 255) / 256 * 256) return;
+  if (blocks && c0 >= ((int64_t)*blocks + 255) / 256 * 256) return;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = i * 32 + t / 8, k = t % 8 * 8;
-    *reinterpret_cast<bf16x8*>(&s_t[r][k]) = *reinterpret_cast<const bf16x8*>(a.hc + (c0 + r) * a.hp + h0 + k);
+    const bool there = c0 + r < rows && h0 + k < cols;
+    *reinterpret_cast<bf16x8*>(&s_t[r][k]) = there ? *reinterpret_cast<const bf16x8*>(src + (c0 + r) * ld_s + h0 + k) : bf16x8{};
   }
   __syncthreads();
 #pragma unroll
@@ -246,7 +250,7 @@ __global__ __launch_bounds__(256) void transpose_kernel(LossArgs a) {
     bf16x8 v;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = s_t[r + e][h];
-    *reinterpret_cast<bf16x8*>(a.hct + (h0 + h) * a.npad + c0 + r) = v;
+    if (h0 + h < cols) *reinterpret_cast<bf16x8*>(dst + (int64_t)(h0 + h) * ld_d + c0 + r) = v;
   }
 }
 
@@ -499,7 +503,8 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
 }
 
 // One wave per row of the caller: joins the row's parts, row loss and lse; rows that do not count get zeros.
-__global__ __launch_bounds__(256) void finish_kernel(LossArgs a, int bm, int bn, int wgs) {
+template <typename C>
+__global__ __launch_bounds__(256) void finish_kernel(LossArgs a, int wgs) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= a.rows) return;
@@ -511,28 +516,29 @@ __global__ __launch_bounds__(256) void finish_kernel(LossArgs a, int bm, int bn,
     }
     return;
   }
-  const int rb = c / bm;
+  // the row block's group: its number, first row block, width; its pairs [gs, ge)
+  const Order O(*a.count, a.vocab, C::BM, C::BN, wgs, 0);
+  const int rb = c / C::BM, full = O.rb >> 3, lslots = 31 - __builtin_clz((unsigned)O.slots);
+  int group = rb >> 3, g0 = group * 8, lw = 3;
+  if (group >= full) {
+    group = full - 1;
+    g0 = full * 8;
+    for (int l = 2; l >= 0; --l)
+      if ((O.rb >> l) & 1) {
+        ++group;
+        lw = l;
+        if (rb < g0 + (1 << l)) break;
+        g0 += 1 << l;
+      }
+  }
+  const int gs = g0 * O.tiles, ge = gs + (O.tiles << lw);
   float m = -3.0e38f, s = 0.f;
-  for (int w = lane; w < wgs; w += 64) {      // the workgroups that had this row block: their first pair of its group
-    const Order O(*a.count, a.vocab, bm, bn, wgs, w / (wgs >> 3));
-    // the group of rb and its pairs
-    const int full = O.rb >> 3;
-    int group = rb >> 3, g0 = group * 8, lw = 3;
-    if (group >= full) {
-      group = full - 1;
-      g0 = full * 8;
-      for (int l = 2; l >= 0; --l)
-        if ((O.rb >> l) & 1) {
-          ++group;
-          lw = l;
-          if (rb < g0 + (1 << l)) break;
-          g0 += 1 << l;
-        }
-    }
-    const int lo = max(g0 * O.tiles, O.base), hi = min(g0 * O.tiles + (O.tiles << lw), O.base + O.cnt);
-    const int t = lo + ((O.base + w % O.slots - lo) & (O.slots - 1));
-    if (t < hi && ((t - g0 * O.tiles) & ((1 << lw) - 1)) == rb - g0) {
-      const float2 o = a.part[(int64_t)(group * wgs + w) * bm + c % bm];
+  for (int w = lane; w < wgs; w += 64) {      // the workgroups that had this row block: they have a pair of its group
+    const int xcd = w >> lslots, q = O.units >> 3, r = O.units & 7;
+    const int base = xcd * q + min(xcd, r), lo = max(gs, base), hi = min(ge, base + q + (xcd < r ? 1 : 0));
+    const int t = lo + ((base + (w & (O.slots - 1)) - lo) & (O.slots - 1));
+    if (t < hi && ((t - gs) & ((1 << lw) - 1)) == rb - g0) {
+      const float2 o = a.part[(int64_t)(group * wgs + w) * C::BM + c % C::BM];
       const float nm = fmaxf(m, o.x);
       s = s * __builtin_amdgcn_exp2f(m - nm) + o.y * __builtin_amdgcn_exp2f(o.x - nm);
       m = nm;
@@ -611,40 +617,50 @@ __device__ __forceinline__ void dlogits_body(const LossArgs& a, char* smem) {
         f32x4 col[C::NI];
 #pragma unroll
         for (int j = 0; j < C::NI; ++j) col[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        typedef VgTurn<C> Turn;
+        const int64_t block = dl_block(a, m0, c0);      // the wave's rows and columns lie in one block
+        const int br = (int)(m0 & 255), bc = c0 & 255;
 #pragma unroll
-        for (int q = 0; q < C::MI; ++q) {
-          const int row = (wm * C::MI + q) * 16 + l16;
-          const float nl = -*reinterpret_cast<const float*>(w + Words<C>::LSE + row * 4), g = *reinterpret_cast<const float*>(w + Words<C>::G + row * 4);
-          f32x4 p[C::NI];
+        for (int q2 = 0; q2 < C::MI / 2; ++q2) {
 #pragma unroll
-          for (int j = 0; j < C::NI; ++j) p[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-          if (g != 0.f) {      // a row of weight 0 has no gradient, whatever its logits are
+          for (int h = 0; h < 2; ++h) {                  // 32 rows x half the columns at a time
 #pragma unroll
-            for (int j = 0; j < C::NI; ++j)
+            for (int u = 0; u < 2; ++u) {
+              const int q = q2 * 2 + u, row = (wm * C::MI + q) * 16 + l16;
+              const float nl = -*reinterpret_cast<const float*>(w + Words<C>::LSE + row * 4), g = *reinterpret_cast<const float*>(w + Words<C>::G + row * 4);
+              f32x4 p[Turn::NJ];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) p[j][e] = g * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[q][j][e], cs, nl));
-            if (label) {
-              const int d = *reinterpret_cast<const int*>(w + Words<C>::Y + row * 4) - n0;
-              if ((unsigned)d < 16u * C::NI && (d & 12) == 0) {
+              for (int j = 0; j < Turn::NJ; ++j) p[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+              if (g != 0.f) {      // a row of weight 0 has no gradient, whatever its logits are
 #pragma unroll
-                for (int j = 0; j < C::NI; ++j)
+                for (int j = 0; j < Turn::NJ; ++j)
 #pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    if (d == j * 16 + e) p[j][e] -= g;
+                  for (int e = 0; e < 4; ++e) p[j][e] = g * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[q][h * Turn::NJ + j][e], cs, nl));
+                if (label) {
+                  const int d = *reinterpret_cast<const int*>(w + Words<C>::Y + row * 4) - n0 - h * Turn::NJ * 16;
+                  if ((unsigned)d < 16u * Turn::NJ && (d & 12) == 0) {
+#pragma unroll
+                    for (int j = 0; j < Turn::NJ; ++j)
+#pragma unroll
+                      for (int e = 0; e < 4; ++e)
+                        if (d == j * 16 + e) p[j][e] -= g;
+                  }
+                }
+              }
+#pragma unroll
+              for (int j = 0; j < Turn::NJ; ++j) {
+                col[h * Turn::NJ + j] += p[j];
+                vg_here(col[h * Turn::NJ + j]);
+                Turn::put(slab, u * 16 + l16, lq, j, p[j]);
               }
             }
+            CACO_WAVE_LDS_SYNC();
+            const int r0 = br + q2 * 32, k0 = bc + h * Turn::NJ * 16;
+            Turn::rows(slab, lane, [&](int r, int ch, bf16x8 v) { vg_stream(a.dl + block + (r0 + r) * 256 + k0 + ch * 8, v); });
+            if (a.dw) Turn::columns(slab, l16, lq, [&](int k, int oct, bf16x8 v) { vg_stream(a.dlt + block + (k0 + k) * 256 + r0 + oct * 8, v); });
+            CACO_WAVE_LDS_SYNC();
+            __builtin_amdgcn_sched_barrier(0);      // one part's registers at a time
           }
-#pragma unroll
-          for (int j = 0; j < C::NI; ++j) {
-            col[j] += p[j];
-            vg_here(col[j]);
-            vg_slab_put<C>(slab, l16, lq, j, p[j]);
-          }
-          CACO_WAVE_LDS_SYNC();
-          bf16_t* d = dl_at(a, m0 + q * 16, c0);      // 16 rows and the wave's columns lie in one block
-          vg_slab_rows<C>(slab, lane, [&](int r, int ch, bf16x8 v) { *reinterpret_cast<bf16x8*>(d + r * 256 + ch * 8) = v; });
-          CACO_WAVE_LDS_SYNC();
-          __builtin_amdgcn_sched_barrier(0);      // one row block's registers at a time
         }
         if (a.db) {
 #pragma unroll
@@ -681,7 +697,10 @@ __global__ __launch_bounds__(256) void targets2_kernel(LossArgs a) {
   const int idx = a.tgt_idx[t], v = idx - a.v0;
   const float g = a.g[c], q = a.tgt_q[t];
   if (idx < 0 || v < 0 || v >= a.piece || g == 0.f || q == 0.f) return;
-  *dl_at(a, c, v) = (bf16_t)(g * __builtin_amdgcn_exp2f(a.tgt_z[t] - a.lse2[c]) - g * q);
+  const bf16_t d = (bf16_t)(g * __builtin_amdgcn_exp2f(a.tgt_z[t] - a.lse2[c]) - g * q);
+  const int64_t block = dl_block(a, c, v);
+  a.dl[block + (c & 255) * 256 + (v & 255)] = d;
+  if (a.dw) a.dlt[block + (v & 255) * 256 + (c & 255)] = d;
   if (!a.db) return;
   const float x = ldexpf(g * q, 38 - fixed_exponent(a));
   if (fabsf(x) <= 0x1p38f) atomicAdd(a.db64 + idx, (unsigned long long)(long long)rintf(x));
@@ -692,6 +711,7 @@ __global__ __launch_bounds__(256) void dbias_kernel(LossArgs a, int bm, int wm) 
   if (c >= a.piece || a.v0 + c >= a.vocab) return;
   const int parts = (*a.count + bm - 1) / bm * wm;
   float s = 0.f;
+#pragma unroll 8
   for (int p = 0; p < parts; ++p) s += a.dbp[(int64_t)p * a.piece + c];
   if (a.topk) s -= (float)ldexp((double)(long long)a.db64[a.v0 + c], fixed_exponent(a) - 38);
   a.db[a.v0 + c] = s;
@@ -712,8 +732,10 @@ struct Share {
   int slice, k0, nkx;              // its slice, the slice's first K-tile and length
   int t0, whole, rest;             // its output tiles: the first, whole ones per workgroup, tiles in the list
   int more, few, many;             // workgroups with a d weight tile more; K-tiles of the list for these and for the others
+  // wgs, ks and with them everything divided by below but `slots - more` are powers of two
   __device__ __forceinline__ Share(const LossArgs& a, int n, int wgs, int xcd) {
     slots = wgs >> 3;
+    const int lslots = 31 - __builtin_clz((unsigned)slots);
     rb = a.dh ? (n + 255) / 256 : 0;
     cb = (a.dim + 255) / 256;
     tiles = rb * cb;
@@ -722,25 +744,22 @@ struct Share {
     const int wt = a.dw ? a.piece / 256 * cb : 0;
     wcnt = (wt >> 3) + (xcd < (wt & 7) ? 1 : 0);
     wbase = xcd * (wt >> 3) + min(xcd, wt & 7);
-    ks = slices(tiles, slots);
-    const int groups = 8 / ks, grp = xcd / ks;
-    slice = xcd % ks;
-    k0 = (int)((int64_t)slice * nk / ks);
-    nkx = (int)((int64_t)(slice + 1) * nk / ks) - k0;
-    t0 = (int)((int64_t)grp * tiles / groups);
-    const int nt = (int)((int64_t)(grp + 1) * tiles / groups) - t0;
-    whole = nt / slots;
-    rest = nt % slots;
-    const int f = wcnt / slots;
-    more = wcnt % slots;
+    int lks = 0;
+    while (lks < 3 && (tiles << lks) < 8 * slots) ++lks;
+    ks = 1 << lks;
+    const int lgroups = 3 - lks, grp = xcd >> lks;
+    slice = xcd & (ks - 1);
+    k0 = (int)(((int64_t)slice * nk) >> lks);
+    nkx = (int)(((int64_t)(slice + 1) * nk) >> lks) - k0;
+    t0 = (int)(((int64_t)grp * tiles) >> lgroups);
+    const int nt = (int)(((int64_t)(grp + 1) * tiles) >> lgroups) - t0;
+    whole = nt >> lslots;
+    rest = nt & (slots - 1);
+    const int f = wcnt >> lslots;
+    more = wcnt & (slots - 1);
     const int list = rest * nkx;   // < slots * 2^18
-    few = max(0, (int)(((int64_t)list + (int64_t)wcnt * nkw + slots - 1) / slots - (int64_t)(f + 1) * nkw));
-    many = max(0, (list - (int)min((int64_t)list, (int64_t)few * more) + slots - more - 1) / (slots - more));
-  }
-  static __host__ __device__ __forceinline__ int slices(int tiles, int slots) {
-    int k = 1;
-    while (k < 8 && tiles * k < 8 * slots) k *= 2;
-    return k;
+    few = max(0, (int)(((list + (int64_t)wcnt * nkw + slots - 1) >> lslots) - (int64_t)(f + 1) * nkw));
+    many = (unsigned)(list - (int)min((int64_t)list, (int64_t)few * more) + slots - more - 1) / (unsigned)(slots - more);
   }
   // first K-tile of workgroup s in the list
   __device__ __forceinline__ int first(int s) const {
@@ -755,6 +774,7 @@ struct Share {
   }
 };
 
+template <bool WT>
 __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
   typedef Big C;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -762,14 +782,14 @@ __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
   const int n = *a.count;
   const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
   const Share S(a, n, gridDim.x, xcd);
-  // d weight: d logits with the token slowest, the transposed hidden states with the token fastest
+  // d weight: both operands with the token fastest
   if (slot < S.wcnt)
-    vg_run<C, true, false, false, false, false>(
+    vg_run<C, false, false, false, false, false>(
         (S.wcnt - slot + S.slots - 1) / S.slots, smem,
         [&](int, int& k0, int& k1) { k0 = 0; k1 = S.nkw; },
         [&](int i) {
           const int tm = (S.wbase + slot + i * S.slots) / S.cb;
-          return VgOperand{a.dl + (int64_t)tm * 65536, 256, C::BM, S.nkw * VG_K, (int64_t)a.piece * 256};
+          return VgOperand{a.dlt + (int64_t)tm * 65536, 256, C::BM, S.nkw * VG_K, (int64_t)a.piece * 256};
         },
         [&](int i) {
           const int c = (S.wbase + slot + i * S.slots) % S.cb * C::BN;
@@ -788,18 +808,18 @@ __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
             CACO_WAVE_LDS_SYNC();
             vg_slab_rows<C>(slab, lane, [&](int r, int ch, bf16x8 v) {
               const int vv = v0 + q * 16 + r, cc = c0 + ch * 8;
-              if (vv < a.vocab && cc < a.dim) *reinterpret_cast<bf16x8*>(a.dw + (int64_t)vv * a.ld_dw + cc) = v;
+              if (vv < a.vocab && cc < a.dim) vg_stream(a.dw + (int64_t)vv * a.ld_dw + cc, v);
             });
             CACO_WAVE_LDS_SYNC();
           }
         });
-  // d hidden: the workgroup's whole tiles, then its part of the list
+  // d hidden: the workgroup's whole tiles, then its part of the list.  The weights as they lie (word slowest), or transposed (WT)
   const int f0 = S.first(slot), f1 = S.first(slot + 1), l0 = f0 < f1 ? f0 / S.nkx : 0;
   const int parts = S.whole + (f0 < f1 ? (f1 - 1) / S.nkx - l0 + 1 : 0);
   if (parts == 0) return;
   const bool first_piece = a.v0 == 0;
   auto out_tile = [&](int i) { return i < S.whole ? S.t0 + slot + i * S.slots : S.t0 + S.whole * S.slots + l0 + i - S.whole; };
-  vg_run<C, false, true, false, false, false>(
+  vg_run<C, false, !WT, false, false, false>(
       parts, smem,
       [&](int i, int& k0, int& k1) {
         const int at = i < S.whole ? 0 : (l0 + i - S.whole) * S.nkx;      // the tile's first K-tile in the list
@@ -809,6 +829,7 @@ __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
       [&](int i) { return VgOperand{a.dl + (int64_t)(out_tile(i) / S.cb) * C::BM * a.piece, 256, C::BM, a.piece, 65536}; },
       [&](int i) {
         const int c = out_tile(i) % S.cb * C::BN;
+        if (WT) return VgOperand{a.wt + (int64_t)c * a.piece, a.piece, a.dim - c, a.piece, 0};
         return VgOperand{a.weight + (int64_t)a.v0 * a.ld_w + c, a.ld_w, a.dim - c, a.vocab - a.v0, 0};
       },
       VgNoWords{}, VgZero{},
@@ -830,9 +851,10 @@ __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
         }
       });
 }
+template <bool WT>
 __global__ __launch_bounds__(Big::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void grads_kernel(LossArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  grads_body(a, smem);
+  grads_body<WT>(a, smem);
 }
 
 // d hidden's parts added in order and rounded once: 16 compact rows x 256 of dim to a workgroup.  It also writes zeros to those of the
@@ -892,7 +914,7 @@ struct Plan {
   int hp, kp;
   int64_t piece;
   bool small;
-  int64_t o_count, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_hct, o_part, o_zt, o_lse2, o_g, o_db64, o_dl, o_slab, o_dbp;
+  int64_t o_count, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_hct, o_part, o_zt, o_lse2, o_g, o_db64, o_dl, o_dlt, o_wt, o_slab, o_dbp;
   int64_t take(int64_t n) {
     const int64_t at = bytes;
     bytes += up(n, 256);
@@ -920,11 +942,14 @@ struct Plan {
     o_lse2 = take(npad * 4);
     o_g = take(npad * 4);
     piece = piece_cols;
-    o_hct = o_db64 = o_dl = o_slab = o_dbp = 0;
+    o_hct = o_db64 = o_dl = o_dlt = o_slab = o_dbp = 0;
+    o_wt = -1;
     if (piece) {
       if (topk) o_db64 = take((int64_t)vocab * 8);
       o_hct = take((int64_t)hp * npad * 2);
       o_dl = take(npad * piece * 2);
+      o_dlt = take(npad * piece * 2);
+      o_wt = rows >= WT_ROWS ? take((int64_t)dim * piece * 2) : -1;
       o_slab = take(Share::slabs(npad / 256 * ((dim + 255) / 256), MAX_CU / 8) * 65536 * 4);
       o_dbp = take(npad / bm * (small ? Small::WM : Big::WM) * piece * 4);
     }
@@ -934,7 +959,7 @@ struct Plan {
 // columns of a piece: the vocabulary in as few equal pieces as d logits of `budget` bytes allow, in whole tiles
 int64_t piece_for(int64_t rows, int vocab, int64_t budget) {
   const int64_t npad = up(rows > 0 ? rows : 1, 256), all = up(vocab, 256);
-  int64_t most = budget / (npad * 2) / 256 * 256;
+  int64_t most = budget / (npad * 4) / 256 * 256;      // two copies
   if (most < 256) most = 256;
   const int64_t pieces = (all + most - 1) / most;
   return up((all + pieces - 1) / pieces, 256);
@@ -960,16 +985,19 @@ int run_loss(LossArgs& a, const Plan& P, int what, int cus, hipStream_t st) {
   if (a.topk) CACO_TRY_RC(launch("loss target logits", target_logits_kernel, pad4, 256, 0, st, a));
   if (fwd) {
     CACO_TRY_RC(launch("loss lse", lse_kernel<C>, dim3(wgs), C::THREADS, C::SMEM_WFAR, st, a));
-    if (a.rows) CACO_TRY_RC(launch("loss finish", finish_kernel, rows4, 256, 0, st, a, (int)C::BM, (int)C::BN, wgs));
+    if (a.rows) CACO_TRY_RC(launch("loss finish", finish_kernel<C>, rows4, 256, 0, st, a, wgs));
     if (a.loss) CACO_TRY_RC(launch("loss reduce", reduce_kernel, dim3(1), 1024, 0, st, a));
   }
   if (!bwd) return CACO_OK;
-  if (a.dw) CACO_TRY_RC(launch("loss transpose", transpose_kernel, dim3((unsigned)(P.npad / 64), a.hp / 64), 256, 0, st, a));
+  if (a.dw) CACO_TRY_RC(launch("loss hidden transpose", transpose_kernel, dim3((unsigned)(P.npad / 64), a.hp / 64), 256, 0, st, (const bf16_t*)a.hc, (int64_t)a.hp, P.npad, a.hp, a.hct, P.npad, (const int*)a.count));
   for (; a.v0 < a.vocab; a.v0 += a.piece) {
     CACO_TRY_RC(launch("loss dlogits", dlogits_kernel<C>, dim3(wgs), C::THREADS, C::SMEM_WFAR, st, a));
     if (a.topk) CACO_TRY_RC(launch("loss targets2", targets2_kernel, dim3((unsigned)(P.npad * a.kp / 256)), 256, 0, st, a));
     if (a.db) CACO_TRY_RC(launch("loss dbias", dbias_kernel, dim3((a.piece + 255) / 256), 256, 0, st, a, (int)C::BM, (int)C::WM));
-    if (a.dh || a.dw) CACO_TRY_RC(launch("loss grads", grads_kernel, dim3(cus), Big::THREADS, Big::SMEM_XFAR, st, a));
+    if (a.dh && a.wt)
+      CACO_TRY_RC(launch("loss weight transpose", transpose_kernel, dim3(a.piece / 64, (a.dim + 63) / 64), 256, 0, st, a.weight + a.v0 * a.ld_w, a.ld_w,
+                         (int64_t)(a.vocab - a.v0), a.dim, a.wt, (int64_t)a.piece, (const int*)nullptr));
+    if (a.dh || a.dw) CACO_TRY_RC(launch("loss grads", a.wt ? grads_kernel<true> : grads_kernel<false>, dim3(cus), Big::THREADS, Big::SMEM_XFAR, st, a));
   }
   if (a.dh && a.rows) CACO_TRY_RC(launch("loss dhidden join", dh_join_kernel, dim3((unsigned)((a.rows + 15) / 16), (a.dim + 255) / 256), 256, 0, st, a, cus));
   return CACO_OK;
@@ -1042,7 +1070,7 @@ int linear_loss(const LinearLoss& c, hipStream_t st) {
   a.count = (int*)(w + P.o_count); a.rowmap = (int*)(w + P.o_rowmap); a.inv = (int*)(w + P.o_inv);
   a.tgt_idx0 = (int*)(w + P.o_ti0); a.tgt_q0 = (float*)(w + P.o_tq0); a.tgt_idx = (int*)(w + P.o_ti); a.tgt_q = (float*)(w + P.o_tq);
   a.hc = (bf16_t*)(w + P.o_hc); a.hct = (bf16_t*)(w + P.o_hct); a.part = (float2*)(w + P.o_part); a.zt = (float*)(w + P.o_zt); a.tgt_z = (float*)(w + P.o_tz); a.lse2 = (float*)(w + P.o_lse2); a.g = (float*)(w + P.o_g);
-  a.dl = (bf16_t*)(w + P.o_dl); a.slab = (float*)(w + P.o_slab); a.dbp = (float*)(w + P.o_dbp);
+  a.dl = (bf16_t*)(w + P.o_dl); a.dlt = (bf16_t*)(w + P.o_dlt); a.wt = P.o_wt >= 0 && c.d_hidden ? (bf16_t*)(w + P.o_wt) : nullptr; a.slab = (float*)(w + P.o_slab); a.dbp = (float*)(w + P.o_dbp);
   a.wmax = (float*)(a.count + 1); a.db64 = (unsigned long long*)(w + P.o_db64);
   a.piece = (int)piece;
   int num_cu = 0;

@@ -31,8 +31,8 @@ Tensor = torch.Tensor
 
 FORWARD, BACKWARD = 1, 2
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
-# d logits of one piece of the vocabulary, bf16: 8192 tokens x 50265 words are one piece, 0.4 % of a card's memory
-PIECE_BYTES = 1 << 30
+# d logits of one piece of the vocabulary, bf16, by rows and by columns: 8192 tokens x 50265 words are one piece, 0.6 % of a card's memory
+PIECE_BYTES = 2 << 30
 
 
 class LinearLossGrads(NamedTuple):

@@ -213,7 +213,7 @@ void caco_decode_end(caco_decode_state* s);
  *   (0 is allowed), vocab <= 2^24, rows * vocab <= 2^46 (both rounded up to 256), dim <= 65536.
  * ws_dev: scratch of the caller's, 16-byte aligned, its contents are not kept; one call at a time may use it.  caco_linear_loss_workspace
  *   gives its size (topk 0 = cross entropy; < 0: CACO_ERR_INVALID); with the backward pass it includes the gradient of the logits
- *   for one piece of the vocabulary in bf16, of about piece_bytes (at least 256 columns).  A smaller workspace makes more pieces.
+ *   for one piece of the vocabulary in bf16, twice, of about piece_bytes together (at least 256 columns).  A smaller workspace makes more pieces.
  * Capturable into a graph: no synchronisation, no allocation, no memset; equal calls give equal bits. */
 #define CACO_LOSS_FORWARD 1
 #define CACO_LOSS_BACKWARD 2
