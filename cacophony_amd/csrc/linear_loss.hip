@@ -13,8 +13,7 @@
 //                part in any product, so whatever its hidden state holds (NaN, infinities) reaches nothing
 //   lse          logits tile by tile; a workgroup stays with a block of rows for many tiles of the vocabulary, every lane keeps a sum of
 //                exp2 over its own columns against a reference that only moves when a sum would leave the range (see lse_body)
-//   finish       row losses in the caller's order, lse: a wave joins the workgroups that shared the row
-//   reduce       their sum or mean in a fixed order
+//   finish       row losses in the caller's order, lse: a wave joins the workgroups that shared the row; their sum or mean in a fixed order
 // and for the gradients, one piece of the vocabulary after the other (as many columns as the workspace holds):
 //   dlogits      the same products again, then g (p - q) rounded to bf16: the operand type of the two products that follow.  The
 //                rounding is 2^-9 of each entry, independent from entry to entry, and the targets are subtracted before it.
@@ -22,7 +21,7 @@
 //   targets2     (distillation) the entries of the teacher's tokens, from the logits that the loss was taken from
 //   grads        d weight's tiles (sums over the tokens, complete) and d hidden (sums over the vocabulary, cut into one run per
 //                workgroup that makes up for the uneven number of d weight's tiles; partial sums are kept in fp32)
-//   dh_join      adds the partial sums in order, one rounding
+//   close        adds d hidden's partial sums and d bias's column sums in order
 // Nothing is accumulated in an order that can change: equal calls give equal bits.
 #define CACO_WAVE_SYNC_FENCE
 #include "common.h"
@@ -62,6 +61,7 @@ struct LossArgs {
   float* db;
   // workspace
   int* count;                        // rows that count
+  unsigned* arrived; double* sums;   // workgroups of `finish` that are through, their sums
   int *rowmap, *inv;                 // compact -> caller's row; caller's row -> compact or -1
   int *tgt_idx0; float *tgt_q0;      // targets in the caller's order [rows, kp] (distillation)
   int *tgt_idx; float *tgt_q;        // targets of the compact rows [npad, kp]
@@ -80,7 +80,7 @@ struct LossArgs {
   bf16_t *dl, *dlt;
   bf16_t* wt;                        // the piece's weights transposed [dim, piece], zeros past the vocabulary; or null
   float* slab;                       // d hidden's partial sums [output tile + workgroup][256][256]
-  float* dbp;                        // [row halves, piece]
+  float* dbp; int64_t vpad;          // column sums of d logits [row halves, vpad = vocabulary rounded up to 256]
   int piece, v0;                     // columns of the piece, its first column
 };
 
@@ -190,6 +190,7 @@ __global__ __launch_bounds__(1024) void compact_kernel(LossArgs a) {
     for (int w = 0; w < 16; ++w) wmax = fmaxf(wmax, s_max[w]);
     *a.wmax = wmax;
     *a.count = at;
+    *a.arrived = 0;
   }
 }
 
@@ -201,42 +202,64 @@ __device__ __forceinline__ float row_gradient(const LossArgs& a, float weight, i
   return g;
 }
 
-// compact row <- its hidden state, targets, gradient scale.  One wave per row; rows up to the next multiple of 256 are zero rows.
+// compact row <- its hidden state (64 rows x 64 of dim to a workgroup, by rows and, for d weight, by columns), targets, gradient scale.
+// Rows up to the next multiple of 256 are zero rows.
 __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, int from_lse) {
-  const int lane = threadIdx.x & 63;
-  const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int n = *a.count;
+  __shared__ bf16_t s_t[64][72];
+  const int t = threadIdx.x, n = *a.count;
+  const int64_t c0 = (int64_t)blockIdx.x * 64;
+  const int h0 = blockIdx.y * 64;
   if (backward && a.db && a.topk)
-    for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < a.vocab; v += (int64_t)gridDim.x * 256) a.db64[v] = 0;
-  if (c >= ((int64_t)n + 255) / 256 * 256) return;
-  const bool real = c < n;
-  const int64_t row = real ? a.rowmap[c] : 0;
-  const bf16x8* src = reinterpret_cast<const bf16x8*>(a.hidden + row * a.ld_h);
-  bf16x8* dst = reinterpret_cast<bf16x8*>(a.hc + c * a.hp);
-  for (int i = lane; i < a.hp / 8; i += 64) dst[i] = real && i < a.dim / 8 ? src[i] : bf16x8{};
-  for (int k = lane; k < a.kp; k += 64) {
+    for (int64_t v = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + t; v < a.vocab; v += (int64_t)gridDim.x * gridDim.y * 256) a.db64[v] = 0;
+  if (c0 >= ((int64_t)n + 255) / 256 * 256) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = i * 32 + t / 8, k = t % 8 * 8;
+    const int64_t c = c0 + r;
+    bf16x8 v = {};
+    if (c < n && h0 + k < a.dim) v = *reinterpret_cast<const bf16x8*>(a.hidden + a.rowmap[c] * a.ld_h + h0 + k);
+    *reinterpret_cast<bf16x8*>(a.hc + c * a.hp + h0 + k) = v;
+    *reinterpret_cast<bf16x8*>(&s_t[r][k]) = v;
+  }
+  if (backward && a.dw) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int h = i * 32 + t / 8, r = t % 8 * 8;
+      bf16x8 v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = s_t[r + e][h];
+      *reinterpret_cast<bf16x8*>(a.hct + (h0 + h) * a.npad + c0 + r) = v;
+    }
+  }
+  const int lkp = 31 - __builtin_clz((unsigned)a.kp);
+  for (int k = blockIdx.y * 256 + t; k < 64 << lkp; k += 256 * gridDim.y) {
+    const int64_t c = c0 + (k >> lkp);
     int idx = -1;
     float q = 0.f;
-    if (real) {
-      idx = a.labels ? (int)a.labels[row] : a.tgt_idx0[row * a.kp + k];
-      q = a.labels ? 1.f : a.tgt_q0[row * a.kp + k];
+    if (c < n) {
+      const int64_t row = a.rowmap[c];
+      const int64_t at = (row << lkp) + (k & (a.kp - 1));
+      idx = a.topk ? a.tgt_idx0[at] : (int)a.labels[row];
+      q = a.topk ? a.tgt_q0[at] : 1.f;
     }
-    a.tgt_idx[c * a.kp + k] = idx;
-    a.tgt_q[c * a.kp + k] = q;
+    a.tgt_idx[c0 * a.kp + k] = idx;
+    a.tgt_q[c0 * a.kp + k] = q;
   }
-  if (backward && lane == 0) {
-    a.g[c] = real ? row_gradient(a, a.row_weight ? a.row_weight[row] : 1.f, n) : 0.f;
-    if (from_lse) a.lse2[c] = real ? a.lse[row] * LOG2E : 0.f;
+  if (backward && blockIdx.y == 0 && t < 64) {
+    const bool real = c0 + t < n;
+    const int64_t row = real ? a.rowmap[c0 + t] : 0;
+    a.g[c0 + t] = real ? row_gradient(a, a.row_weight ? a.row_weight[row] : 1.f, n) : 0.f;
+    if (from_lse) a.lse2[c0 + t] = real ? a.lse[row] * LOG2E : 0.f;
   }
 }
 
-// dst [cols, ld_d] <- src [rows, cols] (ld_s), 64 x 64 at a time through the LDS; rows past the end become zeros, columns past the end (8 of them
-// exist or none) are not written.  `blocks`: if given, only the rows of the first *blocks / 256 (rounded up) blocks of 256 are looked at.
-__global__ __launch_bounds__(256) void transpose_kernel(const bf16_t* src, int64_t ld_s, int64_t rows, int cols, bf16_t* dst, int64_t ld_d, const int* blocks) {
+// The piece's weights by columns: dst [cols, ld_d] <- src [rows, cols] (ld_s), 64 x 64 at a time through the LDS; rows past the end become zeros,
+// columns past the end (8 of them exist or none) are not written.
+__global__ __launch_bounds__(256) void transpose_kernel(const bf16_t* src, int64_t ld_s, int64_t rows, int cols, bf16_t* dst, int64_t ld_d) {
   __shared__ bf16_t s_t[64][72];
   const int64_t c0 = (int64_t)blockIdx.x * 64;
   const int h0 = blockIdx.y * 64, t = threadIdx.x;
-  if (blocks && c0 >= ((int64_t)*blocks + 255) / 256 * 256) return;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = i * 32 + t / 8, k = t % 8 * 8;
@@ -502,19 +525,17 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
   lse_body<C>(a, smem);
 }
 
-// One wave per row of the caller: joins the row's parts, row loss and lse; rows that do not count get zeros.
+// One wave: joins the parts of one of the caller's rows, row loss (returned, too) and lse; rows that do not count get zeros.
 template <typename C>
-__global__ __launch_bounds__(256) void finish_kernel(LossArgs a, int wgs) {
+__device__ __forceinline__ float finish_row(const LossArgs& a, int wgs, int64_t row) {
   const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= a.rows) return;
   const int c = a.inv[row];
   if (c < 0) {
     if (lane == 0) {
-      if (a.row_loss) a.row_loss[row] = 0.f;
+      a.row_loss[row] = 0.f;
       if (a.lse) a.lse[row] = 0.f;
     }
-    return;
+    return 0.f;
   }
   // the row block's group: its number, first row block, width; its pairs [gs, ge)
   const Order O(*a.count, a.vocab, C::BM, C::BN, wgs, 0);
@@ -551,29 +572,49 @@ __global__ __launch_bounds__(256) void finish_kernel(LossArgs a, int wgs) {
     s = s * __builtin_amdgcn_exp2f(m - nm) + os * __builtin_amdgcn_exp2f(om - nm);
     m = nm;
   }
+  const float l2 = m + log2f(s), loss = (l2 - a.zt[c]) * LN2 * a.temperature * a.temperature;
   if (lane == 0) {
-    const float l2 = m + log2f(s);
     a.lse2[c] = l2;
     if (a.lse) a.lse[row] = l2 * LN2;
-    a.row_loss[row] = (l2 - a.zt[c]) * LN2 * a.temperature * a.temperature;
+    a.row_loss[row] = loss;
   }
+  return loss;
 }
 
-// One workgroup, fixed order: sum or mean of the (weighted) row losses.
-__global__ __launch_bounds__(1024) void reduce_kernel(LossArgs a) {
-  __shared__ double s_wave[16];
-  const int tid = threadIdx.x;
-  double s = 0.;
-  for (int64_t r = tid; r < a.rows; r += 1024)
-    if (a.inv[r] >= 0) s += a.row_weight ? (double)a.row_loss[r] * a.row_weight[r] : (double)a.row_loss[r];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if ((tid & 63) == 0) s_wave[tid >> 6] = s;
+// 16 rows to a workgroup.  The sum or mean of the (weighted) row losses: every workgroup leaves its own in `sums`, the last one to arrive
+// adds them in a fixed order.  What passes from one workgroup to another goes past the XCDs' L2s (agent scope), and a workgroup
+// counts itself only after its sum has arrived.
+template <typename C>
+__global__ __launch_bounds__(1024) void finish_kernel(LossArgs a, int wgs) {
+  __shared__ double s_sum[16];
+  __shared__ int s_last;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  double sum = 0.;
+  const int64_t row = (int64_t)blockIdx.x * 16 + wave;
+  if (row < a.rows) {
+    const float l = finish_row<C>(a, wgs, row);
+    if (a.loss && a.inv[row] >= 0) sum = a.row_weight ? (double)l * a.row_weight[row] : (double)l;
+  }
+  if (!a.loss) return;
+  if (lane == 0) s_sum[wave] = sum;
   __syncthreads();
-  if (tid == 0) {
-    double t = 0.;
-    for (int w = 0; w < 16; ++w) t += s_wave[w];
-    *a.loss = (float)(a.reduction == CACO_REDUCE_MEAN ? t / (double)*a.count : t);      // no row counts: 0 / 0, as torch has it
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) sum += s_sum[w];
+    vg_agent_store(a.sums + blockIdx.x, sum);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    s_last = atomicAdd(a.arrived, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  sum = 0.;
+  for (unsigned b = threadIdx.x; b < gridDim.x; b += 1024) sum += vg_agent_load(a.sums + b);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if (lane == 0) s_sum[wave] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) sum += s_sum[w];
+    *a.loss = (float)(a.reduction == CACO_REDUCE_MEAN ? sum / (double)*a.count : sum);      // no row counts: 0 / 0, as torch has it
   }
 }
 
@@ -613,7 +654,7 @@ __device__ __forceinline__ void dlogits_body(const LossArgs& a, char* smem) {
         M.next(O);
         const int64_t m0 = (int64_t)tm * C::BM + wm * 16 * C::MI;
         const int c0 = tn * C::BN + wn * 16 * C::NI;                  // the wave's first column in the piece
-        const int n0 = a.v0 + c0 + lq * 4;                            // this lane's columns: n0 + j * 16 + e
+        const int v0 = a.v0 + c0, n0 = v0 + lq * 4;                   // its word; this lane's columns: n0 + j * 16 + e
         f32x4 col[C::NI];
 #pragma unroll
         for (int j = 0; j < C::NI; ++j) col[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -662,7 +703,7 @@ __device__ __forceinline__ void dlogits_body(const LossArgs& a, char* smem) {
             __builtin_amdgcn_sched_barrier(0);      // one part's registers at a time
           }
         }
-        if (a.db) {
+        if (a.db && v0 < a.vpad) {
 #pragma unroll
           for (int j = 0; j < C::NI; ++j)
 #pragma unroll
@@ -671,7 +712,7 @@ __device__ __forceinline__ void dlogits_body(const LossArgs& a, char* smem) {
               for (int o = 1; o < 16; o <<= 1) col[j][e] += __shfl_xor(col[j][e], o, 64);
           if (l16 == 0)
 #pragma unroll
-            for (int j = 0; j < C::NI; ++j) *reinterpret_cast<f32x4*>(a.dbp + ((int64_t)tm * C::WM + wm) * a.piece + c0 + j * 16 + lq * 4) = col[j];
+            for (int j = 0; j < C::NI; ++j) *reinterpret_cast<f32x4*>(a.dbp + ((int64_t)tm * C::WM + wm) * a.vpad + v0 + j * 16 + lq * 4) = col[j];
         }
       });
 }
@@ -704,17 +745,6 @@ __global__ __launch_bounds__(256) void targets2_kernel(LossArgs a) {
   if (!a.db) return;
   const float x = ldexpf(g * q, 38 - fixed_exponent(a));
   if (fabsf(x) <= 0x1p38f) atomicAdd(a.db64 + idx, (unsigned long long)(long long)rintf(x));
-}
-
-__global__ __launch_bounds__(256) void dbias_kernel(LossArgs a, int bm, int wm) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= a.piece || a.v0 + c >= a.vocab) return;
-  const int parts = (*a.count + bm - 1) / bm * wm;
-  float s = 0.f;
-#pragma unroll 8
-  for (int p = 0; p < parts; ++p) s += a.dbp[(int64_t)p * a.piece + c];
-  if (a.topk) s -= (float)ldexp((double)(long long)a.db64[a.v0 + c], fixed_exponent(a) - 38);
-  a.db[a.v0 + c] = s;
 }
 
 // How a piece's gradient work is shared out, XCD by XCD.
@@ -857,50 +887,72 @@ __global__ __launch_bounds__(Big::THREADS) __attribute__((amdgpu_waves_per_eu(2,
   grads_body<WT>(a, smem);
 }
 
-// d hidden's parts added in order and rounded once: 16 compact rows x 256 of dim to a workgroup.  It also writes zeros to those of the
-// caller's rows with the same numbers that do not count.
-__global__ __launch_bounds__(256) void dh_join_kernel(LossArgs a, int wgs) {
-  __shared__ int64_t s_place[8][MAX_CU / 8 + 1];
-  __shared__ int s_parts[8];
+__device__ __forceinline__ void dbias(const LossArgs& a, int v, int bm, int wm) {
+  if (v >= a.vocab) return;
+  const int parts = (*a.count + bm - 1) / bm * wm;
+  float s = 0.f;
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) s += a.dbp[p * a.vpad + v];
+  if (a.topk) s -= (float)ldexp((double)(long long)a.db64[v], fixed_exponent(a) - 38);
+  a.db[v] = s;
+}
+
+// What is left to add up, in order, once the pieces are through.  The first `joins` workgroups: d hidden's parts, rounded once, 8 compact rows x
+// 256 of dim each, and zeros for those of the caller's rows with the same numbers that do not count.  The others: d bias, 256 words each.
+__global__ __launch_bounds__(256) void close_kernel(LossArgs a, int wgs, int joins, int bm, int wm) {
+  if ((int)blockIdx.x >= joins) {
+    dbias(a, ((int)blockIdx.x - joins) * 256 + threadIdx.x, bm, wm);
+    return;
+  }
+  const int cbs = (a.dim + 255) / 256, by = (int)blockIdx.x % cbs;
+  __shared__ int s_place[8][MAX_CU / 8 + 1], s_parts[8], s_list[8 * (MAX_CU / 8 + 1)];
   const int n = *a.count, t = threadIdx.x;
-  const int64_t c0 = (int64_t)blockIdx.x * 16;
-  const int x = blockIdx.y * 256 + t % 32 * 8;
-  for (int64_t r = c0 + t / 32; r < c0 + 16; r += 8)
-    if (r < a.rows && x < a.dim && a.inv[r] < 0) *reinterpret_cast<bf16x8*>(a.dh + r * a.ld_dh + x) = bf16x8{};
+  const int64_t c0 = (int64_t)((int)blockIdx.x / cbs) * 8, c = c0 + t / 32;
+  const int x = by * 256 + t % 32 * 8;
+  if (c < a.rows && x < a.dim && a.inv[c] < 0) *reinterpret_cast<bf16x8*>(a.dh + c * a.ld_dh + x) = bf16x8{};
   if (c0 >= n) return;
   // where the parts of this output tile are: one thread per XCD
   if (t < 8) {
     const Share S(a, n, wgs, t);
-    const int o = (int)(c0 / 256) * S.cb + blockIdx.y, i = o - S.t0 - S.whole * S.slots;      // the tile's place in the list
+    const int o = (int)(c0 / 256) * S.cb + by, i = o - S.t0 - S.whole * S.slots;      // the tile's place in the list
     int parts = 0;
     if (o >= S.t0 && i < S.rest) {
-      if (i < 0) s_place[t][parts++] = S.slab_whole(o);
+      if (i < 0) s_place[t][parts++] = (int)S.slab_whole(o);
       else
         for (int s = 0; s < S.slots && S.first(s) < (i + 1) * S.nkx; ++s)
-          if (S.first(s + 1) > i * S.nkx && S.first(s + 1) > S.first(s)) s_place[t][parts++] = S.slab_list(t, i, s);
+          if (S.first(s + 1) > i * S.nkx && S.first(s + 1) > S.first(s)) s_place[t][parts++] = (int)S.slab_list(t, i, s);
     }
     s_parts[t] = parts;
   }
   __syncthreads();
-  if (x >= a.dim) return;
-  f32x4 v[2][2] = {};
-  const int r0 = (int)(c0 % 256) + t / 32;
-  for (int xcd = 0; xcd < 8; ++xcd)
-    for (int k = 0; k < s_parts[xcd]; ++k) {
-      const float* p = a.slab + s_place[xcd][k] * 65536 + r0 * 256 + t % 32 * 8;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) v[i][h] += *reinterpret_cast<const f32x4*>(p + i * 8 * 256 + h * 4);
-    }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t c = c0 + t / 32 + i * 8;
-    bf16x8 o8;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o8[e] = (bf16_t)v[i][e / 4][e % 4];
-    if (c < n) *reinterpret_cast<bf16x8*>(a.dh + (int64_t)a.rowmap[c] * a.ld_dh + x) = o8;
+  int parts = 0;
+  for (int xcd = 0; xcd < 8; ++xcd) {
+    if (t < s_parts[xcd]) s_list[parts + t] = s_place[xcd][t];
+    parts += s_parts[xcd];
   }
+  __syncthreads();
+  if (x >= a.dim || c >= n) return;
+  f32x4 v[2] = {};
+  const float* p = a.slab + (c % 256) * 256 + t % 32 * 8;
+  int k = 0;
+  for (; k + 8 <= parts; k += 8) {      // a tile of the list has up to 8 * 32 parts: their loads must not wait for one another
+    f32x4 u[8][2];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) u[j][h] = *reinterpret_cast<const f32x4*>(p + (int64_t)s_list[k + j] * 65536 + h * 4);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) v[h] += u[j][h];
+  }
+  for (; k < parts; ++k)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) v[h] += *reinterpret_cast<const f32x4*>(p + (int64_t)s_list[k] * 65536 + h * 4);
+  bf16x8 o8;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o8[e] = (bf16_t)v[e / 4][e % 4];
+  *reinterpret_cast<bf16x8*>(a.dh + (int64_t)a.rowmap[c] * a.ld_dh + x) = o8;
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
@@ -910,11 +962,11 @@ int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
 // Where everything lies in the workspace.  Sizes are for all `rows`; how many of them count is known on the device only.
 struct Plan {
-  int64_t npad, bytes = 0;
+  int64_t npad, vpad = 0, bytes = 0;
   int hp, kp;
   int64_t piece;
   bool small;
-  int64_t o_count, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_hct, o_part, o_zt, o_lse2, o_g, o_db64, o_dl, o_dlt, o_wt, o_slab, o_dbp;
+  int64_t o_count, o_sums, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_hct, o_part, o_zt, o_lse2, o_g, o_db64, o_dl, o_dlt, o_wt, o_slab, o_dbp;
   int64_t take(int64_t n) {
     const int64_t at = bytes;
     bytes += up(n, 256);
@@ -928,7 +980,8 @@ struct Plan {
     while (kp < topk) kp *= 2;
     small = rows <= Small::BM;
     const int bm = small ? Small::BM : Big::BM;
-    o_count = take(8);                                         // and the largest weight
+    o_count = take(12);                                        // the largest weight, `arrived`
+    o_sums = take(npad / 16 * 8);
     o_rowmap = take(npad * 4);
     o_inv = take(npad * 4);
     o_ti0 = topk ? take(npad * kp * 4) : 0;
@@ -951,7 +1004,8 @@ struct Plan {
       o_dlt = take(npad * piece * 2);
       o_wt = rows >= WT_ROWS ? take((int64_t)dim * piece * 2) : -1;
       o_slab = take(Share::slabs(npad / 256 * ((dim + 255) / 256), MAX_CU / 8) * 65536 * 4);
-      o_dbp = take(npad / bm * (small ? Small::WM : Big::WM) * piece * 4);
+      vpad = up(vocab, 256);
+      o_dbp = take(npad / bm * (small ? Small::WM : Big::WM) * vpad * 4);
     }
   }
 };
@@ -981,25 +1035,24 @@ int run_loss(LossArgs& a, const Plan& P, int what, int cus, hipStream_t st) {
   const bool fwd = what & CACO_LOSS_FORWARD, bwd = what & CACO_LOSS_BACKWARD;
   if (a.topk && a.rows) CACO_TRY_RC(launch("loss targets", targets_kernel, rows4, 256, 0, st, a));
   CACO_TRY_RC(launch("loss compact", compact_kernel, dim3(1), 1024, 0, st, a));
-  CACO_TRY_RC(launch("loss gather", gather_kernel, pad4, 256, 0, st, a, (int)bwd, (int)!fwd));
+  CACO_TRY_RC(launch("loss gather", gather_kernel, dim3((unsigned)(P.npad / 64), a.hp / 64), 256, 0, st, a, (int)bwd, (int)!fwd));
   if (a.topk) CACO_TRY_RC(launch("loss target logits", target_logits_kernel, pad4, 256, 0, st, a));
   if (fwd) {
     CACO_TRY_RC(launch("loss lse", lse_kernel<C>, dim3(wgs), C::THREADS, C::SMEM_WFAR, st, a));
-    if (a.rows) CACO_TRY_RC(launch("loss finish", finish_kernel<C>, rows4, 256, 0, st, a, wgs));
-    if (a.loss) CACO_TRY_RC(launch("loss reduce", reduce_kernel, dim3(1), 1024, 0, st, a));
+    const int64_t fin = (a.rows + 15) / 16;
+    if (a.rows || a.loss) CACO_TRY_RC(launch("loss finish", finish_kernel<C>, dim3((unsigned)(fin ? fin : 1)), 1024, 0, st, a, wgs));
   }
   if (!bwd) return CACO_OK;
-  if (a.dw) CACO_TRY_RC(launch("loss hidden transpose", transpose_kernel, dim3((unsigned)(P.npad / 64), a.hp / 64), 256, 0, st, (const bf16_t*)a.hc, (int64_t)a.hp, P.npad, a.hp, a.hct, P.npad, (const int*)a.count));
   for (; a.v0 < a.vocab; a.v0 += a.piece) {
     CACO_TRY_RC(launch("loss dlogits", dlogits_kernel<C>, dim3(wgs), C::THREADS, C::SMEM_WFAR, st, a));
     if (a.topk) CACO_TRY_RC(launch("loss targets2", targets2_kernel, dim3((unsigned)(P.npad * a.kp / 256)), 256, 0, st, a));
-    if (a.db) CACO_TRY_RC(launch("loss dbias", dbias_kernel, dim3((a.piece + 255) / 256), 256, 0, st, a, (int)C::BM, (int)C::WM));
     if (a.dh && a.wt)
       CACO_TRY_RC(launch("loss weight transpose", transpose_kernel, dim3(a.piece / 64, (a.dim + 63) / 64), 256, 0, st, a.weight + a.v0 * a.ld_w, a.ld_w,
-                         (int64_t)(a.vocab - a.v0), a.dim, a.wt, (int64_t)a.piece, (const int*)nullptr));
+                         (int64_t)(a.vocab - a.v0), a.dim, a.wt, (int64_t)a.piece));
     if (a.dh || a.dw) CACO_TRY_RC(launch("loss grads", a.wt ? grads_kernel<true> : grads_kernel<false>, dim3(cus), Big::THREADS, Big::SMEM_XFAR, st, a));
   }
-  if (a.dh && a.rows) CACO_TRY_RC(launch("loss dhidden join", dh_join_kernel, dim3((unsigned)((a.rows + 15) / 16), (a.dim + 255) / 256), 256, 0, st, a, cus));
+  const int64_t joins = a.dh ? (a.rows + 7) / 8 * ((a.dim + 255) / 256) : 0, words = a.db ? (a.vocab + 255) / 256 : 0;
+  if (joins + words) CACO_TRY_RC(launch("loss close", close_kernel, dim3((unsigned)(joins + words)), 256, 0, st, a, cus, (int)joins, (int)C::BM, (int)C::WM));
   return CACO_OK;
 }
 
@@ -1070,8 +1123,8 @@ int linear_loss(const LinearLoss& c, hipStream_t st) {
   a.count = (int*)(w + P.o_count); a.rowmap = (int*)(w + P.o_rowmap); a.inv = (int*)(w + P.o_inv);
   a.tgt_idx0 = (int*)(w + P.o_ti0); a.tgt_q0 = (float*)(w + P.o_tq0); a.tgt_idx = (int*)(w + P.o_ti); a.tgt_q = (float*)(w + P.o_tq);
   a.hc = (bf16_t*)(w + P.o_hc); a.hct = (bf16_t*)(w + P.o_hct); a.part = (float2*)(w + P.o_part); a.zt = (float*)(w + P.o_zt); a.tgt_z = (float*)(w + P.o_tz); a.lse2 = (float*)(w + P.o_lse2); a.g = (float*)(w + P.o_g);
-  a.dl = (bf16_t*)(w + P.o_dl); a.dlt = (bf16_t*)(w + P.o_dlt); a.wt = P.o_wt >= 0 && c.d_hidden ? (bf16_t*)(w + P.o_wt) : nullptr; a.slab = (float*)(w + P.o_slab); a.dbp = (float*)(w + P.o_dbp);
-  a.wmax = (float*)(a.count + 1); a.db64 = (unsigned long long*)(w + P.o_db64);
+  a.dl = (bf16_t*)(w + P.o_dl); a.dlt = (bf16_t*)(w + P.o_dlt); a.wt = P.o_wt >= 0 && c.d_hidden ? (bf16_t*)(w + P.o_wt) : nullptr; a.slab = (float*)(w + P.o_slab); a.dbp = (float*)(w + P.o_dbp); a.vpad = P.vpad;
+  a.wmax = (float*)(a.count + 1); a.arrived = (unsigned*)(a.count + 2); a.sums = (double*)(w + P.o_sums); a.db64 = (unsigned long long*)(w + P.o_db64);
   a.piece = (int)piece;
   int num_cu = 0;
   CACO_TRY_RC(prepare_launch(reinterpret_cast<const void*>(&lse_kernel<Big>), Big::SMEM_WFAR, &num_cu));

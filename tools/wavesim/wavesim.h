@@ -217,6 +217,7 @@ static inline void __syncthreads() { wavesim::vm_wait(0); wavesim::block_barrier
 static inline int __syncthreads_or(int pred) { wavesim::vm_wait(0); return wavesim::block_barrier_or(pred); }
 
 static inline unsigned long long atomicAdd(unsigned long long* p, unsigned long long v) { return __atomic_fetch_add(p, v, __ATOMIC_RELAXED); }
+static inline unsigned atomicAdd(unsigned* p, unsigned v) { return __atomic_fetch_add(p, v, __ATOMIC_ACQ_REL); }
 static inline unsigned atomicMax(unsigned* p, unsigned v) {
   unsigned o = __atomic_load_n(p, __ATOMIC_RELAXED);
   while (o < v && !__atomic_compare_exchange_n(p, &o, v, false, __ATOMIC_RELAXED, __ATOMIC_RELAXED)) {}
