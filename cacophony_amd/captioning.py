@@ -107,3 +107,25 @@ def decode_caption(model: CACO, tokenizer, audio_batch: Dict[str, torch.Tensor],
     ids = decode_caption_ids(model, audio_batch, max_decode_length, temperature, tokenizer.bos_token_id,
                              tokenizer.eos_token_id, tokenizer.pad_token_id, greedy)
     return tokenizer.batch_decode(ids, skip_special_tokens=True)[0].strip()
+
+
+@torch.no_grad()
+def score_captions(model: CACO, audio_batch: Dict[str, torch.Tensor], text_input_ids, text_mask, captions_per_clip: int = 1):
+    """Log-likelihoods of given captions under the caption decoder: ranks candidate captions of a clip, or measures a captioner.
+    audio_batch = the four tensors of `prepare_audio_batch` for C clips; text_input_ids / text_mask int64 [C * captions_per_clip, T],
+    starting with BOS, a clip's captions one after the other.  Returns (log-likelihood fp32 [C * captions_per_clip], number of scored
+    tokens int64 of the same shape); their quotient is minus the log of the per-token perplexity."""
+    if model.decoder_module is None:
+        raise ValueError("Model does not have a decoder module. Load with use_decoder=True.")     # eval_caco_torch.py:420-421
+    n = int(captions_per_clip)
+    _, audio_hidden = model.get_audio_embedding(audio_batch["audio_patches"], audio_batch["audio_time_inds"],
+                                                audio_batch["audio_freq_inds"], audio_batch["audio_mask"],
+                                                deterministic=True, return_hidden_state=True, normalize=False)
+    audio_mask = _dev_tensor(audio_batch["audio_mask"], torch.float32, model.device, "audio_mask")
+    mask = _dev_tensor(text_mask, torch.int64, model.device, "text_mask")
+    if n < 1 or mask.dim() != 2 or mask.shape[0] != audio_hidden.shape[0] * n:
+        raise ValueError(f"score_captions: {audio_hidden.shape[0]} clips with {n} captions each, got captions {tuple(mask.shape)}")
+    if n > 1:
+        audio_hidden, audio_mask = audio_hidden.repeat_interleave(n, 0), audio_mask.repeat_interleave(n, 0)
+    nll = model.get_caption_nll(audio_hidden, audio_mask, text_input_ids, mask)
+    return -nll.sum(1), (mask[:, 1:] != 0).sum(1)

@@ -1001,36 +1001,40 @@ int caco_encode_text(caco_model* m, const int64_t* ids, const int64_t* mask, int
   return text_forward_impl(m, ids, mask, nullptr, batch, seq, 1, emb, ld_emb, nullptr, stream);
 }
 
-// RobertaDecoder.forward (roberta.py:337-373) as called by CACO.get_decoder_logits (caco.py:212-240): teacher-forced
-// logits over the vocabulary for every caption position, cross-attending to the audio encoder's hidden states.
-int caco_decoder_forward(caco_model* m, const float* text_hidden, const int64_t* text_mask, const float* audio_hidden,
-                         const float* audio_mask, int32_t batch, int32_t seq_t, int32_t seq_a, float* logits, void* stream) {
+// RobertaDecoder.forward (roberta.py:337-373) as called by CACO.get_decoder_logits (caco.py:212-240), up to the hidden states of its
+// last layer: teacher-forced, cross-attending to the audio encoder's hidden states.
+struct DecoderWs {
+  size_t x, y, xb, qkv, o, a, mask, ab, kv;
+  DecoderWs(Arena& A, int64_t M, int64_t Ma, int H, int I) {
+    x = A.reserve((size_t)M * H * 4); y = A.reserve((size_t)M * H * 4); xb = A.reserve((size_t)M * H * 2);
+    qkv = A.reserve((size_t)M * qkv_ld(H) * 2); o = A.reserve((size_t)M * H * 2); a = A.reserve((size_t)M * I * 2);
+    mask = A.reserve((size_t)M * 4); ab = A.reserve((size_t)Ma * H * 2); kv = A.reserve((size_t)Ma * 2 * H * 2);
+  }
+};
+static int check_decoder(caco_model* m, const void* text_hidden, const void* text_mask, const void* audio_hidden, const void* audio_mask, const void* out,
+                         int32_t batch, int32_t seq_t, int32_t seq_a, const char* what) {
   CACO_REQUIRE(m && m->finalized, "model is null or weights not finalized");
   CACO_TRY(check_device(m));
   CACO_REQUIRE(!m->dlayers.empty() && m->dec_proj.w, "Decoder module not initialized");
-  CACO_REQUIRE(text_hidden && text_mask && audio_hidden && audio_mask && logits && batch > 0 && seq_t > 0 && seq_a > 0,
-               "caco_decoder_forward: bad arguments");
+  CACO_REQUIRE(text_hidden && text_mask && audio_hidden && audio_mask && out && batch > 0 && seq_t > 0 && seq_a > 0, "%s: bad arguments", what);
+  return CACO_OK;
+}
+// leaves the hidden states in the arena, bf16 [batch * seq_t, H] at w.xb
+static int run_decoder(caco_model* m, const Arena& A, const DecoderWs& w, const float* text_hidden, const int64_t* text_mask, const float* audio_hidden,
+                       const float* audio_mask, int32_t batch, int32_t seq_t, int32_t seq_a, hipStream_t st) {
   const caco_config& c = m->cfg;
-  hipStream_t st = (hipStream_t)stream;
-  const int H = c.text_hidden, I = c.text_intermediate, V = c.text_vocab, Vp = m->dec_proj.out;
+  const int H = c.text_hidden;
   const int heads = c.text_heads, hd = H / heads;
   const int64_t M = (int64_t)batch * seq_t, Ma = (int64_t)batch * seq_a;
-  Arena A(m, WS_TEXT, st);
-  const size_t o_x = A.reserve((size_t)M * H * 4), o_y = A.reserve((size_t)M * H * 4), o_xb = A.reserve((size_t)M * H * 2);
-  const size_t o_qkv = A.reserve((size_t)M * qkv_ld(H) * 2), o_o = A.reserve((size_t)M * H * 2), o_a = A.reserve((size_t)M * I * 2);
-  const size_t o_mask = A.reserve((size_t)M * 4), o_ab = A.reserve((size_t)Ma * H * 2), o_kv = A.reserve((size_t)Ma * 2 * H * 2);
-  const size_t o_lg = A.reserve((size_t)M * Vp * 4);
-  CACO_TRY(A.commit(st));
-  float* x = A.at<float>(o_x);
-  float* y = A.at<float>(o_y);
-  bf16_t* xb = A.at<bf16_t>(o_xb);
-  bf16_t* qkv = A.at<bf16_t>(o_qkv);
-  bf16_t* o = A.at<bf16_t>(o_o);
-  bf16_t* a = A.at<bf16_t>(o_a);
-  float* fmask = A.at<float>(o_mask);
-  bf16_t* ab = A.at<bf16_t>(o_ab);
-  bf16_t* kv = A.at<bf16_t>(o_kv);
-  float* lg = A.at<float>(o_lg);
+  float* x = A.at<float>(w.x);
+  float* y = A.at<float>(w.y);
+  bf16_t* xb = A.at<bf16_t>(w.xb);
+  bf16_t* qkv = A.at<bf16_t>(w.qkv);
+  bf16_t* o = A.at<bf16_t>(w.o);
+  bf16_t* a = A.at<bf16_t>(w.a);
+  float* fmask = A.at<float>(w.mask);
+  bf16_t* ab = A.at<bf16_t>(w.ab);
+  bf16_t* kv = A.at<bf16_t>(w.kv);
   CACO_TRY(mask_i64_to_f32(text_mask, fmask, M, st));
   CACO_HIP(hipMemcpyAsync(x, text_hidden, (size_t)M * H * 4, hipMemcpyDeviceToDevice, st));
   CACO_STAGE("decoder.cast", cast_f32_to_bf16(x, xb, M * H, st));
@@ -1052,9 +1056,49 @@ int caco_decoder_forward(caco_model* m, const float* text_hidden, const int64_t*
     CACO_STAGE("decoder.gemm_fc2", linear_f32(L.t.out, a, M, x, y, st));
     CACO_STAGE("decoder.ln", layernorm(y, L.t.ln_out.g, L.t.ln_out.b, M, H, c.text_ln_eps, x, xb, st));
   }
+  return CACO_OK;
+}
+
+int caco_decoder_forward(caco_model* m, const float* text_hidden, const int64_t* text_mask, const float* audio_hidden,
+                         const float* audio_mask, int32_t batch, int32_t seq_t, int32_t seq_a, float* logits, void* stream) {
+  CACO_TRY(check_decoder(m, text_hidden, text_mask, audio_hidden, audio_mask, logits, batch, seq_t, seq_a, "caco_decoder_forward"));
+  const caco_config& c = m->cfg;
+  hipStream_t st = (hipStream_t)stream;
+  const int H = c.text_hidden, V = c.text_vocab, Vp = m->dec_proj.out;
+  const int64_t M = (int64_t)batch * seq_t, Ma = (int64_t)batch * seq_a;
+  Arena A(m, WS_TEXT, st);
+  const DecoderWs w(A, M, Ma, H, c.text_intermediate);
+  const size_t o_lg = A.reserve((size_t)M * Vp * 4);
+  CACO_TRY(A.commit(st));
+  float* lg = A.at<float>(o_lg);
+  CACO_TRY(run_decoder(m, A, w, text_hidden, text_mask, audio_hidden, audio_mask, batch, seq_t, seq_a, st));
   // decoder_proj (roberta.py:371): [M, H] x [Vp, H]^T into the padded scratch rows, then the V real columns out
-  CACO_STAGE("decoder.gemm_vocab", linear_f32(m->dec_proj, xb, M, nullptr, lg, st));
+  CACO_STAGE("decoder.gemm_vocab", linear_f32(m->dec_proj, A.at<bf16_t>(w.xb), M, nullptr, lg, st));
   CACO_HIP(hipMemcpy2DAsync(logits, (size_t)V * 4, lg, (size_t)Vp * 4, (size_t)V * 4, (size_t)M, hipMemcpyDeviceToDevice, st));
+  return CACO_OK;
+}
+
+// The same up to the likelihoods of given tokens: the vocabulary's logits exist a tile at a time only (linear_loss.hip).
+int caco_decoder_score(caco_model* m, const float* text_hidden, const int64_t* text_mask, const float* audio_hidden, const float* audio_mask,
+                       const int64_t* targets, int64_t ignore_index, int32_t batch, int32_t seq_t, int32_t seq_a, float* nll, void* stream) {
+  CACO_TRY(check_decoder(m, text_hidden, text_mask, audio_hidden, audio_mask, nll, batch, seq_t, seq_a, "caco_decoder_score"));
+  CACO_REQUIRE(targets, "caco_decoder_score: bad arguments");
+  const caco_config& c = m->cfg;
+  hipStream_t st = (hipStream_t)stream;
+  const int H = c.text_hidden;
+  const int64_t M = (int64_t)batch * seq_t, Ma = (int64_t)batch * seq_a;
+  const int64_t ws_bytes = linear_loss_workspace(M, c.text_vocab, H, 0, 0, CACO_LOSS_FORWARD);
+  if (ws_bytes < 0) return CACO_ERR_INVALID;
+  Arena A(m, WS_TEXT, st);
+  const DecoderWs w(A, M, Ma, H, c.text_intermediate);
+  const size_t o_ws = A.reserve((size_t)ws_bytes);
+  CACO_TRY(A.commit(st));
+  CACO_TRY(run_decoder(m, A, w, text_hidden, text_mask, audio_hidden, audio_mask, batch, seq_t, seq_a, st));
+  LinearLoss l{};
+  l.what = CACO_LOSS_FORWARD; l.hidden = A.at<bf16_t>(w.xb); l.ld_h = H; l.weight = m->dec_proj.w; l.ld_w = H; l.bias = m->dec_proj.b;
+  l.labels = targets; l.ignore_index = ignore_index; l.rows = M; l.vocab = c.text_vocab; l.dim = H;
+  l.row_loss = nll; l.ws = A.at<char>(o_ws); l.ws_bytes = ws_bytes;
+  CACO_STAGE("decoder.score", linear_loss(l, st));
   return CACO_OK;
 }
 

@@ -15,8 +15,10 @@
 //                exp2 over its own columns against a reference that only moves when a sum would leave the range (see lse_body)
 //   finish       row losses in the caller's order, lse: a wave joins the workgroups that shared the row; their sum or mean in a fixed order
 // and for the gradients, one piece of the vocabulary after the other (as many columns as the workspace holds):
-//   dlogits      the same products again, then g (p - q) rounded to bf16: the operand type of the two products that follow.  The
-//                rounding is 2^-9 of each entry, independent from entry to entry, and the targets are subtracted before it.
+//   dlogits      the same products again, then g (p - q), g the row's weight, rounded to bf16: the operand type of the two products that
+//                follow.  The rounding is at most 2^-8 of each entry (2^-9 on average), and the targets are subtracted before it.  What all rows
+//                have in common (T, the incoming gradient, 1 / count) waits for the fp32 results: inside the entries it would round
+//                1 - p of every confident row alike, an error that does not average out over the rows.
 //                Column sums for d bias are taken from the unrounded values.
 //   targets2     (distillation) the entries of the teacher's tokens, from the logits that the loss was taken from
 //   grads        d weight's tiles (sums over the tokens, complete) and d hidden (sums over the vocabulary, cut into one run per
@@ -70,7 +72,7 @@ struct LossArgs {
   float2* part;                      // (max, sum) of log2-logits, [group of row blocks][workgroup][rows of a block]
   float* zt;                         // cross entropy: the label's log2-logit; distillation: sum_k q_k (z_k / T - log q_k), log2 units
   float* tgt_z;                      // distillation: the entries' log2-logits [npad, kp]
-  float *lse2, *g;                   // compact: lse in log2 units, gradient scale of the row
+  float *lse2, *g;                   // compact: lse in log2 units, the row's weight in the gradients
   float* wmax;                       // largest |row_weight| of the rows that count
   unsigned long long* db64;          // distillation: sum of the targets' weights per word, fixed point in units of 2^(e - 38), |g| < 2^e
   // d logits of the piece in blocks of 256 rows x 256 columns, [row block][column block][256][256], once with the columns next to one another
@@ -194,15 +196,16 @@ __global__ __launch_bounds__(1024) void compact_kernel(LossArgs a) {
   }
 }
 
-// T from the logits' scale and the loss's T^2, the row's weight, the incoming gradient, the mean
-__device__ __forceinline__ float row_gradient(const LossArgs& a, float weight, int n) {
-  float g = a.temperature * weight;
+// what the gradients of all n rows have in common: T from the logits' scale and the loss's T^2, the incoming gradient, the mean
+__device__ __forceinline__ float common_scale(const LossArgs& a, int n) {
+  if (n == 0) return 0.f;
+  float g = a.temperature;
   if (a.grad_scale) g *= *a.grad_scale;
   if (a.reduction == CACO_REDUCE_MEAN) g /= (float)n;
   return g;
 }
 
-// compact row <- its hidden state (64 rows x 64 of dim to a workgroup, by rows and, for d weight, by columns), targets, gradient scale.
+// compact row <- its hidden state (64 rows x 64 of dim to a workgroup, by rows and, for d weight, by columns), targets, weight.
 // Rows up to the next multiple of 256 are zero rows.
 __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, int from_lse) {
   __shared__ bf16_t s_t[64][72];
@@ -249,7 +252,7 @@ __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, i
   if (backward && blockIdx.y == 0 && t < 64) {
     const bool real = c0 + t < n;
     const int64_t row = real ? a.rowmap[c0 + t] : 0;
-    a.g[c0 + t] = real ? row_gradient(a, a.row_weight ? a.row_weight[row] : 1.f, n) : 0.f;
+    a.g[c0 + t] = real && common_scale(a, n) != 0.f ? a.row_weight ? a.row_weight[row] : 1.f : 0.f;
     if (from_lse) a.lse2[c0 + t] = real ? a.lse[row] * LOG2E : 0.f;
   }
 }
@@ -722,15 +725,15 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
   dlogits_body<C>(a, smem);
 }
 
-// exponent e of the fixed point: every |g| < 2^e, because row_gradient grows with |weight| (0 where the largest is not finite or is zero)
+// exponent e of the fixed point: every |g| < 2^e (0 where the largest is not finite or is zero)
 __device__ __forceinline__ int fixed_exponent(const LossArgs& a) {
-  const unsigned m = __float_as_uint(fabsf(row_gradient(a, *a.wmax, *a.count)));
+  const unsigned m = __float_as_uint(*a.wmax);
   return m == 0 || m >= 0x7f800000u ? 0 : max((int)(m >> 23), 1) - 126;
 }
 
 // (distillation) d logits at the teacher's tokens of the piece: one thread per entry.  The tokens of a row are distinct, so an entry is
 // written by one thread.  Their share of d bias is added as 64-bit integers, whose sum does not depend on the order: an entry is below
-// 2^38 units (q <= 1), the 2^24 rows' sum below 2^62, and a unit is 2^-38 of the largest |g|.
+// 2^38 units (q <= 1), the 2^22 rows' sum below 2^62, and a unit is 2^-38 of the largest |g|.
 __global__ __launch_bounds__(256) void targets2_kernel(LossArgs a) {
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t c = t / a.kp;
@@ -811,6 +814,7 @@ __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
   const int wm = wave / C::WN, wn = wave % C::WN;
   const int n = *a.count;
   const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+  const float scale = common_scale(a, n);
   const Share S(a, n, gridDim.x, xcd);
   // d weight: both operands with the token fastest
   if (slot < S.wcnt)
@@ -834,7 +838,7 @@ __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
 #pragma unroll
           for (int q = 0; q < C::MI; ++q) {
 #pragma unroll
-            for (int j = 0; j < C::NI; ++j) vg_slab_put<C>(slab, l16, lq, j, acc[q][j]);
+            for (int j = 0; j < C::NI; ++j) vg_slab_put<C>(slab, l16, lq, j, acc[q][j] * scale);
             CACO_WAVE_LDS_SYNC();
             vg_slab_rows<C>(slab, lane, [&](int r, int ch, bf16x8 v) {
               const int vv = v0 + q * 16 + r, cc = c0 + ch * 8;
@@ -894,7 +898,7 @@ __device__ __forceinline__ void dbias(const LossArgs& a, int v, int bm, int wm) 
 #pragma unroll 8
   for (int p = 0; p < parts; ++p) s += a.dbp[p * a.vpad + v];
   if (a.topk) s -= (float)ldexp((double)(long long)a.db64[v], fixed_exponent(a) - 38);
-  a.db[v] = s;
+  a.db[v] = s * common_scale(a, *a.count);
 }
 
 // What is left to add up, in order, once the pieces are through.  The first `joins` workgroups: d hidden's parts, rounded once, 8 compact rows x
@@ -949,9 +953,10 @@ __global__ __launch_bounds__(256) void close_kernel(LossArgs a, int wgs, int joi
   for (; k < parts; ++k)
 #pragma unroll
     for (int h = 0; h < 2; ++h) v[h] += *reinterpret_cast<const f32x4*>(p + (int64_t)s_list[k] * 65536 + h * 4);
+  const float scale = common_scale(a, n);
   bf16x8 o8;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) o8[e] = (bf16_t)v[e / 4][e % 4];
+  for (int e = 0; e < 8; ++e) o8[e] = (bf16_t)(v[e / 4][e % 4] * scale);
   *reinterpret_cast<bf16x8*>(a.dh + (int64_t)a.rowmap[c] * a.ld_dh + x) = o8;
 }
 
@@ -1011,10 +1016,16 @@ struct Plan {
 };
 
 // columns of a piece: the vocabulary in as few equal pieces as d logits of `budget` bytes allow, in whole tiles
+// The 256 rows of a tile are addressed from its first one with 32 bits: 255 strides of bf16 stay below 2^31.  The strides are `dim`,
+// the weight's, and in the transposed operands the rows (padded) and the piece.
+constexpr int64_t MAX_LD = (int64_t)1 << 22;
+static_assert(255 * MAX_LD * 2 + VG_K * 2 < 0x7fffffff, "a tile's last row lies within its descriptor");
+
 int64_t piece_for(int64_t rows, int vocab, int64_t budget) {
   const int64_t npad = up(rows > 0 ? rows : 1, 256), all = up(vocab, 256);
   int64_t most = budget / (npad * 4) / 256 * 256;      // two copies
   if (most < 256) most = 256;
+  if (most > MAX_LD) most = MAX_LD;
   const int64_t pieces = (all + most - 1) / most;
   return up((all + pieces - 1) / pieces, 256);
 }
@@ -1059,7 +1070,7 @@ int run_loss(LossArgs& a, const Plan& P, int what, int cus, hipStream_t st) {
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 int check_sizes(int64_t rows, int32_t vocab, int32_t dim, int32_t topk) {
-  CACO_REQUIRE(rows >= 0 && rows <= (int64_t)1 << 24, "linear loss: rows must be 0 .. 2^24, got %lld", (long long)rows);
+  CACO_REQUIRE(rows >= 0 && rows <= MAX_LD, "linear loss: rows must be 0 .. 2^22, got %lld", (long long)rows);
   CACO_REQUIRE(vocab >= 1 && vocab <= 1 << 24, "linear loss: vocab must be 1 .. 2^24, got %d", vocab);
   CACO_REQUIRE(dim >= 8 && dim <= 1 << 16 && dim % 8 == 0, "linear loss: dim must be a multiple of 8 in 8 .. 65536, got %d", dim);
   CACO_REQUIRE(up(rows, 256) * up(vocab, 256) <= (int64_t)1 << 46, "linear loss: rows * vocab must not exceed 2^46, got %lld * %d", (long long)rows, vocab);
@@ -1080,12 +1091,13 @@ int linear_loss(const LinearLoss& c, hipStream_t st) {
   CACO_REQUIRE(c.reduction >= CACO_REDUCE_NONE && c.reduction <= CACO_REDUCE_SUM, "linear loss: unknown reduction %d", c.reduction);
   CACO_REQUIRE(c.weight && c.ws && (c.rows == 0 || (c.hidden && (c.topk ? c.teacher && c.teacher_idx : c.labels != nullptr))), "linear loss: null argument");
   CACO_REQUIRE(c.topk == 0 || (c.temperature > 0.f && c.temperature < INFINITY), "linear loss: temperature must be positive and finite");
+  CACO_REQUIRE(c.topk == 0 || (c.temperature >= 0x1p-20f && c.temperature <= 0x1p20f), "linear loss: temperature must be within 2^-20 .. 2^20, got %g", (double)c.temperature);
   const bool fwd = c.what & CACO_LOSS_FORWARD, bwd = c.what & CACO_LOSS_BACKWARD;
   CACO_REQUIRE(!fwd || c.rows == 0 || c.row_loss, "linear loss: the forward pass needs row_loss");
   CACO_REQUIRE(!c.loss || (fwd && c.reduction != CACO_REDUCE_NONE), "linear loss: a reduced loss needs the forward pass and a reduction");
   CACO_REQUIRE(fwd || c.rows == 0 || c.lse, "linear loss: the backward pass alone needs the forward pass's lse");
   CACO_REQUIRE(!bwd || c.d_hidden || c.d_weight || c.d_bias, "linear loss: the backward pass has no output");
-  CACO_REQUIRE(c.ld_h >= c.dim && c.ld_h % 8 == 0 && c.ld_w >= c.dim && c.ld_w % 8 == 0 && c.ld_w < 1 << 22 && aligned16(c.hidden) && aligned16(c.weight),
+  CACO_REQUIRE(c.ld_h >= c.dim && c.ld_h % 8 == 0 && c.ld_w >= c.dim && c.ld_w % 8 == 0 && c.ld_w < MAX_LD && aligned16(c.hidden) && aligned16(c.weight),
                "linear loss: rows of hidden and weight must start at multiples of 16 bytes (strides >= dim, multiples of 8)");
   CACO_REQUIRE(!bwd || ((!c.d_hidden || (c.ld_dh >= c.dim && c.ld_dh % 8 == 0 && aligned16(c.d_hidden))) &&
                         (!c.d_weight || (c.ld_dw >= c.dim && c.ld_dw % 8 == 0 && aligned16(c.d_weight)))),
@@ -1096,7 +1108,7 @@ int linear_loss(const LinearLoss& c, hipStream_t st) {
   int64_t piece = 0;
   if (bwd) {
     const int64_t all = up(c.vocab, 256);
-    int64_t lo = 1, hi = all / 256;                      // in tiles; the plan's size grows with the piece
+    int64_t lo = 1, hi = (all < MAX_LD ? all : MAX_LD) / 256;      // in tiles; the plan's size grows with the piece
     CACO_REQUIRE(Plan(c.rows, c.vocab, c.dim, c.topk, 256).bytes <= c.ws_bytes, "linear loss: the workspace is too small (caco_linear_loss_workspace)");
     while (lo < hi) {
       const int64_t mid = (lo + hi + 1) / 2;

@@ -82,7 +82,7 @@ class _Head:
 
 def _rows(x: Tensor) -> Tuple[Tensor, int]:
     """[n, dim] whose rows start at multiples of 16 bytes, and their stride."""
-    if x.stride(1) != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) < x.shape[1] or x.stride(0) % 8)):
+    if x.stride(1) != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) < x.shape[1] or x.stride(0) % 8 or x.stride(0) >= 1 << 22)):
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
@@ -146,14 +146,15 @@ class _LinearLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, head, target, ignore_index, piece_bytes):
         out, lse = _forward(head, target, ignore_index, True)
-        ctx.save_for_backward(hidden, weight, bias)      # the tensors themselves: a change in place before the backward pass is an error
+        # the tensors themselves (a detached one shares their version): a change in place before the backward pass is an error
+        ctx.save_for_backward(hidden, weight, bias, *(t for t in target.values() if torch.is_tensor(t)))
         ctx.head, ctx.target, ctx.lse, ctx.ignore_index, ctx.piece_bytes = head, target, lse, ignore_index, piece_bytes
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        hidden, weight, bias = ctx.saved_tensors
+        hidden, weight, bias = ctx.saved_tensors[:3]
         head = ctx.head
         with torch.cuda.device(head.device):
             new = lambda n, t: torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and ctx.needs_input_grad[n] else None
@@ -213,7 +214,7 @@ def linear_topk_distillation(hidden: Tensor, weight: Tensor, teacher_logits: Ten
     """T^2 KL(q || softmax(z / T)) with z = hidden @ weight.T + bias and q = softmax(teacher_logits / T) over the entries a teacher gives
     per row: teacher_logits [..., k], teacher_indices int32 or int64 [..., k], k <= 128 (`retrieval.topk` or `torch.topk` of the teacher's
     logits).  An index outside [0, vocab) (`retrieval.topk` pads with -1) or a logit of -inf is no entry, entries of one token add up, a
-    row without entries has loss 0 and does not count."""
+    row without entries has loss 0 and does not count.  temperature 2^-20 .. 2^20."""
     head = _Head("linear_topk_distillation", hidden, weight, bias, reduction)
     return _loss(head, _teacher(head, teacher_logits, teacher_indices, temperature), hidden, weight, bias, -100, piece_bytes)
 

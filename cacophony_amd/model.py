@@ -228,9 +228,7 @@ class CACO(_HipModel):
         at = similarity(a, t, float(torch.exp(self.logit_scale)))
         return at, at.T
 
-    def _decoder_forward(self, text_hidden_state, attention_mask, audio_hidden_state, audio_mask, deterministic: bool = True):
-        """RobertaDecoder.forward (text_models/roberta.py:337-373): [B,T,H], [B,T], [B,S,H], [B,S] -> logits [B,T,vocab]."""
-        self._inference_only(deterministic)
+    def _decoder_operands(self, text_hidden_state, attention_mask, audio_hidden_state, audio_mask):
         th = _dev_tensor(text_hidden_state, torch.float32, self.device, "text_hidden_state")
         tm = _dev_tensor(attention_mask, torch.int64, self.device, "attention_mask")
         ah = _dev_tensor(audio_hidden_state, torch.float32, self.device, "audio_hidden_state")
@@ -242,6 +240,12 @@ class CACO(_HipModel):
         S = ah.shape[1]
         if tuple(tm.shape) != (B, T) or tuple(am.shape) != (B, S):
             raise ValueError(f"decoder: masks must be [{B}, {T}] and [{B}, {S}], got {tuple(tm.shape)} / {tuple(am.shape)}")
+        return th, tm, ah, am, B, T, S
+
+    def _decoder_forward(self, text_hidden_state, attention_mask, audio_hidden_state, audio_mask, deterministic: bool = True):
+        """RobertaDecoder.forward (text_models/roberta.py:337-373): [B,T,H], [B,T], [B,S,H], [B,S] -> logits [B,T,vocab]."""
+        self._inference_only(deterministic)
+        th, tm, ah, am, B, T, S = self._decoder_operands(text_hidden_state, attention_mask, audio_hidden_state, audio_mask)
         logits = torch.empty(B, T, self.text_config.vocab_size, dtype=torch.float32, device=self.device)
         with torch.cuda.device(self.device):
             _lib.check(self._lib.caco_decoder_forward(self._handle, _ptr(th), _ptr(tm), _ptr(ah), _ptr(am), B, T, S,
@@ -255,6 +259,27 @@ class CACO(_HipModel):
         _, text_hidden_state = self.get_text_embedding(text_input_ids=text_input_ids, text_mask=text_mask,
                                                        deterministic=deterministic)
         return self._decoder_forward(text_hidden_state, text_mask, audio_hidden_state, audio_mask, deterministic)
+
+    def get_caption_nll(self, audio_hidden_state, audio_mask, text_input_ids, text_mask, deterministic: bool = True) -> Tensor:
+        """-log p(token t + 1 | tokens 0 .. t, audio) of given captions, fp32 [B, T - 1]: the cross entropy of
+        `get_decoder_logits(...)[:, :-1]` with `text_input_ids[:, 1:]`, 0 where text_mask[:, 1:] is 0.  The logits are not formed
+        (C ABI: caco_decoder_score); `captioning.score_captions` sums it per caption."""
+        if self.decoder_module is None:
+            raise ValueError("Decoder module not initialized")      # caco.py:223-224
+        self._inference_only(deterministic)
+        ids = _dev_tensor(text_input_ids, torch.int64, self.device, "text_input_ids")
+        mask = _dev_tensor(text_mask, torch.int64, self.device, "text_mask")
+        if ids.dim() != 2 or ids.shape != mask.shape or ids.shape[1] < 2:
+            raise ValueError(f"text_input_ids / text_mask must both be [B, T >= 2], got {tuple(ids.shape)} / {tuple(mask.shape)}")
+        self._check_token_ids(ids, None)
+        _, text_hidden_state = self.get_text_embedding(ids[:, :-1], mask[:, :-1], check_ids=False)
+        th, tm, ah, am, B, T, S = self._decoder_operands(text_hidden_state, mask[:, :-1], audio_hidden_state, audio_mask)
+        targets = torch.where(mask[:, 1:] != 0, ids[:, 1:], -100).contiguous()
+        nll = torch.empty(B, T, dtype=torch.float32, device=self.device)
+        with torch.cuda.device(self.device):
+            _lib.check(self._lib.caco_decoder_score(self._handle, _ptr(th), _ptr(tm), _ptr(ah), _ptr(am), _ptr(targets), -100, B, T, S,
+                                                    _ptr(nll), _stream()), "caption_nll")
+        return nll
 
     def forward(self, audio_patches, audio_time_inds, audio_freq_inds, audio_mask, text_input_ids, text_mask,
                 deterministic: bool = True):

@@ -176,6 +176,13 @@ int caco_decoder_forward(caco_model* m, const float* text_hidden_dev, const int6
                          const float* audio_hidden_dev, const float* audio_mask_dev, int32_t batch, int32_t seq_text,
                          int32_t seq_audio, float* logits_dev, void* stream);
 
+/* ... and the likelihoods of given tokens instead of the logits: nll_dev fp32 [B, T] = -log softmax(logits[b, t])[targets[b, t]], 0 where
+ * targets_dev int64 [B, T] is ignore_index or outside the vocabulary.  The reference has the logits only (caco.py:212-240); scoring 256
+ * captions of 32 tokens through them takes 3.2 GB of logits, this call about 0.2 GB of scratch. */
+int caco_decoder_score(caco_model* m, const float* text_hidden_dev, const int64_t* text_mask_dev, const float* audio_hidden_dev,
+                       const float* audio_mask_dev, const int64_t* targets_dev, int64_t ignore_index, int32_t batch, int32_t seq_text,
+                       int32_t seq_audio, float* nll_dev, void* stream);
+
 /* ---- incremental caption decoding with key / value caches: the JAX path's get_next_decoder_logits loop
  * (src/caco/caco.py:154-230; the torch path re-runs the whole prefix every step, eval_caco_torch.py:443-456).
  * caco_decode_begin projects the audio hidden states to every decoder layer's cross-attention keys / values once and
@@ -202,6 +209,7 @@ void caco_decode_end(caco_decode_state* s);
  *   [rows, topk] (ld_t), teacher_idx_dev int32 or int64 (idx_bytes 4 or 8) [rows, topk] (ld_i).  q = softmax(teacher / T) over the row's
  *   entries, row loss = T^2 * sum_k q_k (log q_k - log softmax(z / T)[i_k]).  An index outside [0, vocab) (caco_topk pads with -1) or a
  *   logit of -inf is no entry; entries of one token add up; a row without entries does not count.
+ *   2^-20 <= T <= 2^20.
  * `what`: CACO_LOSS_FORWARD writes row_loss_dev fp32 [rows], lse_dev fp32 [rows] (logsumexp of z, of z / T for the distillation; may be
  *   NULL when the backward pass is not a later call) and, for a reduction other than CACO_REDUCE_NONE, loss_dev fp32 [1] (may be NULL) = sum of
  *   row_weight * row_loss, divided for CACO_REDUCE_MEAN by the number of rows that count (NaN if none does).  CACO_LOSS_BACKWARD
@@ -209,7 +217,7 @@ void caco_decode_end(caco_decode_state* s);
  *   [rows, dim] (ld_dh), d_weight_dev bf16 [vocab, dim] (ld_dw), d_bias_dev fp32 [vocab]; each may be NULL, not all.  It reads lse_dev
  *   unless the forward pass is part of the same call (CACO_LOSS_FORWARD | CACO_LOSS_BACKWARD).  No row counts: zero gradients.
  *   row_weight_dev fp32 [rows] or NULL (= 1), grad_scale_dev fp32 [1] or NULL (= 1).
- * Row strides are in elements, >= dim and multiples of 8, and rows start at multiples of 16 bytes; dim is a multiple of 8; rows <= 2^24
+ * Row strides are in elements, >= dim and multiples of 8, and rows start at multiples of 16 bytes; dim is a multiple of 8; rows <= 2^22
  *   (0 is allowed), vocab <= 2^24, rows * vocab <= 2^46 (both rounded up to 256), dim <= 65536.
  * ws_dev: scratch of the caller's, 16-byte aligned, its contents are not kept; one call at a time may use it.  caco_linear_loss_workspace
  *   gives its size (topk 0 = cross entropy; < 0: CACO_ERR_INVALID); with the backward pass it includes the gradient of the logits

@@ -1,0 +1,131 @@
+"""Likelihoods of given captions (caco_decoder_score, CACO.get_caption_nll, captioning.score_captions): the caption decoder's hidden
+states through the linear cross entropy, checked against the cross entropy of the logits the decoder gives for the same captions
+(src/caco_torch/caco.py:212-240) and against the reference's own logits."""
+import ctypes as C
+from dataclasses import replace
+
+import numpy as np
+import pytest
+import torch
+
+from cacophony_amd import _lib, config, synth
+from tests.conftest import load_golden
+
+
+def _configs():
+    a, t, cc = config.tiny_configs(2)
+    return a, t, cc, replace(t, num_hidden_layers=2)
+
+
+@pytest.fixture(scope="module")
+def model():
+    from cacophony_amd.model import CACO
+    a, t, cc, d = _configs()
+    return CACO(a, t, cc, decoder_config=d, device="cuda:0").load_state_dict(synth.make_caco_state(a, t, cc, seed=0, decoder_cfg=d))
+
+
+@pytest.fixture(scope="module")
+def clips(model):
+    from cacophony_amd import frontend
+    ab = frontend.mel_patches_device(torch.from_numpy(synth.make_waveforms(2, start=40)).cuda(), 500, torch.float32)
+    _, ah = model.get_audio_embedding(ab["audio_patches"], ab["audio_time_inds"], ab["audio_freq_inds"], ab["audio_mask"])
+    return ab, ah
+
+
+def nll_of(logits, ids, mask):
+    """fp64 [B, T - 1] from logits of the first T - 1 tokens"""
+    lp = torch.log_softmax(logits.double().cpu(), -1)
+    return torch.where(torch.as_tensor(mask)[:, 1:] != 0, -lp.gather(2, torch.as_tensor(ids)[:, 1:, None])[..., 0], 0.0)
+
+
+def test_refused_without_a_model():
+    lib = _lib.load()
+    one = C.c_void_p(1024)
+    assert lib.caco_decoder_score(None, one, one, one, one, one, -100, 1, 1, 1, one, None) == _lib.CACO_ERR_INVALID
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,start", [(2, 40), (9, 7), (33, 100)])
+def test_nll_is_the_cross_entropy_of_the_decoders_logits(model, clips, n, start):
+    """Same hidden states, bit for bit, on both sides; what differs is the order in which 768 products are added up in fp32, at most
+    768 * 2^-24 of the sum of their magnitudes (below 10 here: layer-normed states times 0.02 weights) and twice that for
+    logsumexp minus logit: 1e-3."""
+    ab, ah = clips
+    V = model.text_config.vocab_size
+    ids, mask = synth.make_captions(n, 32, V, start=start)
+    pick = torch.arange(n, device="cuda") % 2
+    ah, am = ah[pick], ab["audio_mask"][pick]
+    nll = model.get_caption_nll(ah, am, ids, mask)
+    assert nll.shape == (n, 31) and nll.dtype == torch.float32
+    want = nll_of(model.get_decoder_logits(ah, am, ids[:, :-1], mask[:, :-1]), ids, mask)
+    assert (nll.cpu().double() - want).abs().max() < 1e-3
+    assert not nll.cpu()[torch.as_tensor(mask)[:, 1:] == 0].any()
+    assert torch.equal(nll, model.get_caption_nll(ah, am, ids, mask))
+
+
+@pytest.mark.gpu
+def test_nll_against_the_references_logits(model, clips):
+    """bf16 operands against the reference's fp32: the logits' bar is rel-L2 1e-2; a row's logits have 2-norm |z|, so a logit is off by
+    at most 1e-2 |z| and its likelihood by twice that."""
+    g = load_golden("decoder_tiny.npz")
+    ab, ah = clips
+    nll = model.get_caption_nll(ah, ab["audio_mask"], g["ids"], g["tmask"]).cpu().double()
+    z = torch.from_numpy(g["logits"][:, :-1])
+    bound = 2e-2 * z.double().norm(dim=-1)
+    assert ((nll - nll_of(z, g["ids"], g["tmask"])).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+def test_smallest_and_padded_captions(model, clips):
+    ab, ah = clips
+    am = ab["audio_mask"]
+    ids = torch.tensor([[0, 17], [0, 4]])
+    nll = model.get_caption_nll(ah, am, ids, torch.ones_like(ids))
+    want = nll_of(model.get_decoder_logits(ah, am, ids[:, :1], torch.ones(2, 1)), ids, torch.ones_like(ids))
+    assert nll.shape == (2, 1) and (nll.cpu().double() - want).abs().max() < 1e-3
+    # a caption of which only BOS exists has no likelihood to add; the other's stays as it is, whatever lies behind its end
+    ids, mask = synth.make_captions(2, 16, model.text_config.vocab_size, start=3)
+    mask = mask.copy()
+    mask[0, 1:] = 0
+    mask[1, 9:] = 0
+    other = ids.copy()
+    other[:, 9:] = 5
+    one, two = model.get_caption_nll(ah, am, ids, mask), model.get_caption_nll(ah, am, other, mask)
+    assert not one[0].any() and not one[1, 8:].any() and one[1, :8].all() and torch.equal(one[1], two[1])
+
+
+@pytest.mark.gpu
+def test_score_captions_ranks_a_clips_candidates(model, clips):
+    from cacophony_amd import captioning
+    ab, ah = clips
+    ids, mask = synth.make_captions(6, 24, model.text_config.vocab_size, start=60)
+    score, count = captioning.score_captions(model, ab, ids, mask, captions_per_clip=3)
+    assert score.shape == count.shape == (6,) and count.cpu().tolist() == (mask[:, 1:] != 0).sum(1).tolist()
+    for c in range(2):
+        for i in range(3):
+            r = 3 * c + i
+            lg = model.get_decoder_logits(ah[c:c + 1], ab["audio_mask"][c:c + 1], ids[r:r + 1, :-1], mask[r:r + 1, :-1])
+            want = -nll_of(lg, ids[r:r + 1], mask[r:r + 1]).sum()
+            assert abs(float(score[r]) - float(want)) < 2e-2 * abs(float(want)) + 1e-3      # other row counts, other GEMM tiles: bf16 roundings of the states
+    with pytest.raises(ValueError, match="3 captions"):
+        captioning.score_captions(model, ab, ids[:5], mask[:5], captions_per_clip=3)
+    with pytest.raises(ValueError, match=r"T >= 2"):
+        model.get_caption_nll(ah, ab["audio_mask"], ids[:2, :1], mask[:2, :1])
+    with pytest.raises(ValueError):
+        model.get_caption_nll(ah[:1], ab["audio_mask"][:1], ids[:2], mask[:2])
+    bad = ids.copy()
+    bad[0, 3] = model.text_config.vocab_size
+    with pytest.raises((ValueError, IndexError)):
+        model.get_caption_nll(ah, ab["audio_mask"], bad[:2], mask[:2])
+
+
+@pytest.mark.gpu
+def test_models_without_a_decoder_refuse(tiny_state):
+    from cacophony_amd import captioning
+    from cacophony_amd.model import CACO
+    a, t, cc, _ = _configs()
+    plain = CACO(a, t, cc, device="cuda:0").load_state_dict(tiny_state)
+    with pytest.raises(ValueError, match="Decoder module not initialized"):
+        plain.get_caption_nll(torch.zeros(1, 8, 768), torch.ones(1, 8), torch.zeros(1, 4, dtype=torch.long), torch.ones(1, 4))
+    with pytest.raises(ValueError, match="use_decoder=True"):
+        captioning.score_captions(plain, {}, torch.zeros(1, 4, dtype=torch.long), torch.ones(1, 4))

@@ -189,7 +189,7 @@ def _ce(lib, **kw):
 @pytest.mark.parametrize("change,message", [
     (dict(what=0), b"what"), (dict(what=4), b"what"), (dict(reduction=3), b"reduction"), (dict(reduction=-1), b"reduction"),
     (dict(hidden=None), b"null"), (dict(weight=None), b"null"), (dict(labels=None), b"null"), (dict(ws=None), b"null"),
-    (dict(rows=-1), b"rows"), (dict(rows=2 ** 24 + 1), b"rows"), (dict(vocab=0), b"vocab"), (dict(vocab=2 ** 24 + 1), b"vocab"),
+    (dict(rows=-1), b"rows"), (dict(rows=2 ** 24 + 1), b"rows"), (dict(rows=2 ** 22 + 1), b"rows"), (dict(vocab=0), b"vocab"), (dict(vocab=2 ** 24 + 1), b"vocab"),
     (dict(dim=0), b"dim"), (dict(dim=60), b"dim"), (dict(dim=65544), b"dim"), (dict(row_loss=None), b"row_loss"), (dict(reduction=0), b"reduced loss"),
     (dict(what=2, loss=None, lse=None), b"lse"), (dict(dh=None, dw=None, db=None), b"no output"),
     (dict(ld_h=56), b"16 bytes"), (dict(ld_h=65), b"16 bytes"), (dict(ld_w=56), b"16 bytes"), (dict(ld_w=68), b"16 bytes"), (dict(ld_w=1 << 22), b"16 bytes"),
@@ -208,7 +208,7 @@ def test_distillation_calls_that_are_refused():
     def call(topk=4, T=1.0, nbytes=8, ld_t=4, ld_i=4, teacher=1024, idx=1024):
         return lib.caco_linear_distill(3, 1024, 64, 1024, 64, None, teacher, ld_t, idx, ld_i, nbytes, topk, T, 4, 300, 64, 1, None, None, 1024, 1024, 1024,
                                        1024, 64, 1024, 64, 1024, 1024, 0, None)
-    for kw in (dict(topk=0), dict(topk=129, ld_t=129, ld_i=129), dict(T=0.0), dict(T=-1.0), dict(T=math.inf), dict(T=math.nan), dict(nbytes=2), dict(ld_t=3),
+    for kw in (dict(topk=0), dict(topk=129, ld_t=129, ld_i=129), dict(T=0.0), dict(T=-1.0), dict(T=math.inf), dict(T=math.nan), dict(T=2.0 ** -21), dict(T=2.0 ** 21), dict(T=1e-40), dict(nbytes=2), dict(ld_t=3),
                dict(ld_i=3), dict(teacher=None), dict(idx=None), dict()):
         assert call(**kw) == _lib.CACO_ERR_INVALID, kw
     assert b"too small" in lib.caco_last_error()
@@ -221,6 +221,10 @@ def test_workspace_sizes():
     fwd, one, many = size(8192, 50265, 768, 0, 1 << 30, 1), size(8192, 50265, 768, 0, 1 << 30, 3), size(8192, 50265, 768, 0, 1, 3)
     assert 0 < fwd < many < one and one < 2 << 30 and fwd < 32 << 20
     assert size(8192, 50265, 768, 128, 1 << 30, 1) > fwd
+    # 255 strides of a transposed operand are addressed with 31 bits: no piece has more than 2^22 columns, however much memory there is
+    all_of_it = 2 * 2 * 256 * 2 ** 24
+    assert size(1, 2 ** 24, 8, 0, 1 << 50, 3) < size(1, 2 ** 22, 8, 0, 1 << 50, 3) + (size(1, 2 ** 24, 8, 0, 1, 3) - size(1, 2 ** 22, 8, 0, 1, 3)) + (1 << 20) < all_of_it
+    assert size(2 ** 22, 50265, 768, 0, 1 << 30, 3) > 0 > size(2 ** 22 + 1, 50265, 768, 0, 1 << 30, 3)
 
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="exercises the no-GPU failure mode")
@@ -464,6 +468,22 @@ def test_captured_and_replayed_between_eager_calls(topk):
             for a, b in zip(o1, e):
                 assert torch.equal(a, b)
             assert torch.equal(o2, e.row_loss)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["h", "w", "b", "y", "teacher", "idx"])
+def test_an_operand_changed_before_the_backward_pass_is_an_error(name):
+    from cacophony_amd import losses
+    d = dev(make(20, 150, 64, topk=3, seed=41))
+    h = d["h"].clone().requires_grad_()
+    if name == "y":
+        loss = losses.linear_cross_entropy(h, d["w"], d["y"], d["b"])
+    else:
+        loss = losses.linear_topk_distillation(h, d["w"], d["teacher"], d["idx"], d["b"])
+    with torch.no_grad():
+        (h if name == "h" else d[name]).zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
 
 
 @pytest.mark.gpu
