@@ -474,7 +474,7 @@ def test_captured_and_replayed_between_eager_calls(topk):
 @pytest.mark.parametrize("name", ["h", "w", "b", "y", "teacher", "idx"])
 def test_an_operand_changed_before_the_backward_pass_is_an_error(name):
     from cacophony_amd import losses
-    d = dev(make(20, 150, 64, topk=3, seed=41))
+    d = dev(make(20, 150, 64, topk=0 if name == "y" else 3, seed=41))
     h = d["h"].clone().requires_grad_()
     if name == "y":
         loss = losses.linear_cross_entropy(h, d["w"], d["y"], d["b"])
