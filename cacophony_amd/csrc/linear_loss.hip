@@ -70,7 +70,7 @@ struct LossArgs {
   bf16_t* hc;                        // [npad, hp]
   bf16_t* hct;                       // [hp, npad]: its transpose, for d weight
   float2* part;                      // (max, sum) of log2-logits, [group of row blocks][workgroup][rows of a block]
-  float* zt;                         // cross entropy: the label's log2-logit; distillation: sum_k q_k (z_k / T - log q_k), log2 units
+  float* zt;                         // cross entropy: the label's logit; distillation: sum_k q_k (z_k / T - log q_k), log2 units
   float* tgt_z;                      // distillation: the entries' log2-logits [npad, kp]
   float *lse2, *g;                   // compact: lse in log2 units, the row's weight in the gradients
   float* wmax;                       // largest |row_weight| of the rows that count
@@ -92,8 +92,8 @@ struct LossArgs {
 // One wave per row: q = softmax(t / T) over the entries whose index lies in the vocabulary; an index that occurs again adds its weight
 // to its first place.  A row without entries gets none (all indices -1).
 __global__ __launch_bounds__(256) void targets_kernel(LossArgs a) {
-  __shared__ int s_idx[4][128];
-  __shared__ float s_q[4][128];
+  __shared__ __attribute__((aligned(16))) int s_idx[4][128];
+  __shared__ __attribute__((aligned(16))) float s_q[4][128];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = (int64_t)blockIdx.x * 4 + wave;
   if (row >= a.rows) return;      // a wave keeps to its own part of the LDS: no barrier follows
@@ -132,12 +132,19 @@ __global__ __launch_bounds__(256) void targets_kernel(LossArgs a) {
     const int k = h * 64 + lane;
     float q = 0.f;
     int out = idx[h];
-    if (out >= 0)
-      for (int o = 0; o < a.topk; ++o)
-        if (s_idx[wave][o] == out) {
-          if (o < k) { out = -1; break; }
-          q += s_q[wave][o];
-        }
+    bool again = false;
+    // every entry against every other, four at a time and without a branch, so that the reads do not wait for one another
+    for (int o = 0; o < a.topk; o += 4) {
+      typedef int i32x4 __attribute__((ext_vector_type(4)));
+      const i32x4 si = *reinterpret_cast<const i32x4*>(&s_idx[wave][o]);
+      const f32x4 sq = *reinterpret_cast<const f32x4*>(&s_q[wave][o]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        again |= si[e] == out && o + e < k;
+        q += si[e] == out ? sq[e] : 0.f;
+      }
+    }
+    if (again) out = -1;
     if (k < a.kp) {
       a.tgt_idx0[row * a.kp + k] = out;
       a.tgt_q0[row * a.kp + k] = out < 0 ? 0.f : q;
@@ -281,37 +288,53 @@ __global__ __launch_bounds__(256) void transpose_kernel(const bf16_t* src, int64
 }
 
 // (distillation) sum_k q_k (log q_k - z_k / T) of a compact row: 16 lanes per entry, the entries' rows of weight gathered.
-// Also in log2 units, so that `finish` treats both losses alike.
+// In log2 units, as `finish` has them.  A row with 16 entries or more has four waves: what it takes is the gathers' latency, and one wave
+// after the other through 100 entries took 61 us for 1000 rows, four waves TL_US.
+constexpr int target_waves(int kp) { return kp >= 16 ? 4 : 1; }
 __global__ __launch_bounds__(256) void target_logits_kernel(LossArgs a) {
-  const int lane = threadIdx.x & 63, l16 = lane & 15, grp = lane >> 4;
-  const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (c >= *a.count) return;
-  const bf16_t* h = a.hc + c * a.hp;
+  __shared__ float s_sum[4];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, grp = lane >> 4, wave = threadIdx.x >> 6;
+  const int waves = target_waves(a.kp), part = wave & (waves - 1);
+  const int64_t c = waves == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  const bool real = c < *a.count;
   float sum = 0.f;
-  for (int k0 = 0; k0 < a.kp; k0 += 4) {
-    const int k = k0 + grp;
-    const int idx = k < a.kp ? a.tgt_idx[c * a.kp + k] : -1;
-    const float q = k < a.kp ? a.tgt_q[c * a.kp + k] : 0.f;
-    float z = 0.f;
-    if (idx >= 0) {
-      const bf16_t* w = a.weight + (int64_t)idx * a.ld_w;
-      for (int i = l16 * 8; i < a.dim; i += 128) {
-        const bf16x8 x = *reinterpret_cast<const bf16x8*>(h + i), y = *reinterpret_cast<const bf16x8*>(w + i);
+  if (real) {
+    const bf16_t* h = a.hc + c * a.hp;
+    const int share = a.kp / waves;                       // up to 32 entries of this wave, in steps of four
+    const int at = l16 * 4 + grp;                         // lane (step, group) brings that step's entry of the group: all of them at once
+    const int64_t first = c * a.kp + part * share;
+    const int idx0 = at < share ? a.tgt_idx[first + at] : -1;
+    const float q0 = at < share ? a.tgt_q[first + at] : 0.f;
+    const int steps = (share + 3) / 4;
+    for (int s = 0; s < steps; ++s) {
+      const int idx = __shfl(idx0, grp * 16 + s, 64);
+      const float q = __shfl(q0, grp * 16 + s, 64);
+      float z = 0.f;
+      if (idx >= 0) {
+        const bf16_t* w = a.weight + (int64_t)idx * a.ld_w;
+        for (int i = l16 * 8; i < a.dim; i += 128) {
+          const bf16x8 x = *reinterpret_cast<const bf16x8*>(h + i), y = *reinterpret_cast<const bf16x8*>(w + i);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z = __builtin_fmaf((float)x[e], (float)y[e], z);
+          for (int e = 0; e < 8; ++e) z = __builtin_fmaf((float)x[e], (float)y[e], z);
+        }
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
+      if (q != 0.f && l16 == 0) {      // 0 log 0 = 0: an entry of weight 0 (or none) adds nothing, whatever its logit is
+        if (a.bias) z += a.bias[idx];
+        z *= a.inv_t * LOG2E;
+        sum += q * (log2f(q) - z);
+        a.tgt_z[first + s * 4 + grp] = z;
       }
     }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
-    if (q != 0.f && l16 == 0) {      // 0 log 0 = 0: an entry of weight 0 (or none) adds nothing, whatever its logit is
-      if (a.bias) z += a.bias[idx];
-      z *= a.inv_t * LOG2E;
-      sum += q * (log2f(q) - z);
-      a.tgt_z[c * a.kp + k] = z;
-    }
+    sum = wave_sum(sum);
   }
-  sum = wave_sum(sum);
-  if (lane == 0) a.zt[c] = -sum;
+  if (lane == 0) s_sum[wave] = sum;
+  __syncthreads();
+  if (real && lane == 0 && part == 0) {
+    if (waves == 4) sum = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+    a.zt[c] = -sum;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
@@ -483,7 +506,7 @@ __device__ __forceinline__ void lse_body(const LossArgs& a, char* smem) {
               for (int j = 0; j < C::NI; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                  if (d == j * 16 + e) zy = acc[q][j][e] * cs;
+                  if (d == j * 16 + e) zy = acc[q][j][e];
               a.zt[(int64_t)rb * C::BM + row] = zy;
             }
           }
@@ -575,7 +598,9 @@ __device__ __forceinline__ float finish_row(const LossArgs& a, int wgs, int64_t 
     s = s * __builtin_amdgcn_exp2f(m - nm) + os * __builtin_amdgcn_exp2f(om - nm);
     m = nm;
   }
-  const float l2 = m + log2f(s), loss = (l2 - a.zt[c]) * LN2 * a.temperature * a.temperature;
+  // the target is taken from the reference first: what a confident row loses is not rounded at the logits' size
+  const float ls = log2f(s), l2 = m + ls, d = a.topk ? m - a.zt[c] : __builtin_fmaf(-a.zt[c], a.inv_t * LOG2E, m);
+  const float loss = (d + ls) * LN2 * a.temperature * a.temperature;
   if (lane == 0) {
     a.lse2[c] = l2;
     if (a.lse) a.lse[row] = l2 * LN2;
@@ -1047,7 +1072,7 @@ int run_loss(LossArgs& a, const Plan& P, int what, int cus, hipStream_t st) {
   if (a.topk && a.rows) CACO_TRY_RC(launch("loss targets", targets_kernel, rows4, 256, 0, st, a));
   CACO_TRY_RC(launch("loss compact", compact_kernel, dim3(1), 1024, 0, st, a));
   CACO_TRY_RC(launch("loss gather", gather_kernel, dim3((unsigned)(P.npad / 64), a.hp / 64), 256, 0, st, a, (int)bwd, (int)!fwd));
-  if (a.topk) CACO_TRY_RC(launch("loss target logits", target_logits_kernel, pad4, 256, 0, st, a));
+  if (a.topk) CACO_TRY_RC(launch("loss target logits", target_logits_kernel, target_waves(a.kp) == 4 ? dim3((unsigned)P.npad) : pad4, 256, 0, st, a));
   if (fwd) {
     CACO_TRY_RC(launch("loss lse", lse_kernel<C>, dim3(wgs), C::THREADS, C::SMEM_WFAR, st, a));
     const int64_t fin = (a.rows + 15) / 16;
