@@ -8,7 +8,7 @@
 //
 // A call, in launches:
 //   targets      (distillation) the teacher's softmax per row; entries of one token are merged; rows with no entry do not count
-//   compact      row numbers of the rows that count, in order; how many
+//   compact      row numbers of the rows that count, in order; how many (64 rows or fewer: part of `gather`)
 //   gather       those rows of `hidden`, next to one another, padded with zero rows and columns: a row that does not count takes no
 //                part in any product, so whatever its hidden state holds (NaN, infinities) reaches nothing
 //   lse          logits tile by tile; a workgroup stays with a block of rows for many tiles of the vocabulary, every lane keeps a sum of
@@ -65,6 +65,7 @@ struct LossArgs {
   int* count;                        // rows that count
   unsigned* arrived; double* sums;   // workgroups of `finish` that are through, their sums
   int *rowmap, *inv;                 // compact -> caller's row; caller's row -> compact or -1
+  int* some;                         // distillation: caller's row has an entry
   int *tgt_idx0; float *tgt_q0;      // targets in the caller's order [rows, kp] (distillation)
   int *tgt_idx; float *tgt_q;        // targets of the compact rows [npad, kp]
   bf16_t* hc;                        // [npad, hp]
@@ -150,7 +151,7 @@ __global__ __launch_bounds__(256) void targets_kernel(LossArgs a) {
       a.tgt_q0[row * a.kp + k] = out < 0 ? 0.f : q;
     }
   }
-  if (lane == 0) a.inv[row] = some;                        // for `compact`
+  if (lane == 0) a.some[row] = some;
 }
 
 // the 256 x 256 block of d logits that holds (row, col)
@@ -162,8 +163,11 @@ __device__ __forceinline__ bool row_counts(const LossArgs& a, int64_t r) {
     const int64_t y = a.labels[r];
     return y != a.ignore_index && y >= 0 && y < a.vocab;
   }
-  return a.inv[r] != 0;
+  return a.some[r] != 0;
 }
+
+// up to this many rows are counted by every workgroup of `gather` for itself, which saves `compact` and its launch (3.5 us of 35)
+constexpr int FEW_ROWS = 64;
 
 // One workgroup: every wave counts a run of consecutive rows, 64 at a time; a scan over the waves gives each run its first place.
 // Also the largest |row_weight| of the rows that count.
@@ -182,7 +186,7 @@ __global__ __launch_bounds__(1024) void compact_kernel(LossArgs a) {
   float wmax = a.row_weight ? 0.f : 1.f;
   for (int64_t r = r0; r < r1; r += 64) {
     const int64_t row = r + lane;
-    const bool c = row < r1 && row_counts(a, min(row, r1 - 1));      // this wave's own rows: read before they are overwritten
+    const bool c = row < r1 && row_counts(a, min(row, r1 - 1));
     const unsigned long long mask = __ballot(c);
     const int place = at + __builtin_popcountll(mask & ((1ull << lane) - 1));
     if (row < r1) a.inv[row] = c ? place : -1;
@@ -214,10 +218,36 @@ __device__ __forceinline__ float common_scale(const LossArgs& a, int n) {
 
 // compact row <- its hidden state (64 rows x 64 of dim to a workgroup, by rows and, for d weight, by columns), targets, weight.
 // Rows up to the next multiple of 256 are zero rows.
+// FEW: `compact` has not run.  Every wave counts the call's rows, one lane each, and the first workgroup writes down what `compact` does.
+template <bool FEW>
 __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, int from_lse) {
   __shared__ bf16_t s_t[64][72];
-  const int t = threadIdx.x, n = *a.count;
+  __shared__ int s_row[FEW ? FEW_ROWS : 1];
+  const int t = threadIdx.x;
   const int64_t c0 = (int64_t)blockIdx.x * 64;
+  int n;
+  if (FEW) {
+    const int r = t & 63;
+    const bool c = r < a.rows && row_counts(a, r);
+    const unsigned long long mask = __ballot(c);
+    n = __builtin_popcountll(mask);
+    const int place = __builtin_popcountll(mask & ((1ull << r) - 1));
+    if (t < 64 && c) s_row[place] = r;
+    if (t < 64 && blockIdx.x == 0 && blockIdx.y == 0) {
+      if (r < a.rows) a.inv[r] = c ? place : -1;
+      if (c) a.rowmap[place] = r;
+      const float wmax = wave_max(!a.row_weight ? 1.f : c ? fabsf(a.row_weight[r]) : 0.f);
+      if (r == 0) {
+        *a.wmax = wmax;
+        *a.count = n;
+        *a.arrived = 0;
+      }
+    }
+    __syncthreads();
+  } else {
+    n = *a.count;
+  }
+  const int* rowmap = FEW ? s_row : a.rowmap;
   const int h0 = blockIdx.y * 64;
   if (backward && a.db && a.topk)
     for (int64_t v = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + t; v < a.vocab; v += (int64_t)gridDim.x * gridDim.y * 256) a.db64[v] = 0;
@@ -227,7 +257,7 @@ __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, i
     const int r = i * 32 + t / 8, k = t % 8 * 8;
     const int64_t c = c0 + r;
     bf16x8 v = {};
-    if (c < n && h0 + k < a.dim) v = *reinterpret_cast<const bf16x8*>(a.hidden + a.rowmap[c] * a.ld_h + h0 + k);
+    if (c < n && h0 + k < a.dim) v = *reinterpret_cast<const bf16x8*>(a.hidden + rowmap[c] * a.ld_h + h0 + k);
     *reinterpret_cast<bf16x8*>(a.hc + c * a.hp + h0 + k) = v;
     *reinterpret_cast<bf16x8*>(&s_t[r][k]) = v;
   }
@@ -248,7 +278,7 @@ __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, i
     int idx = -1;
     float q = 0.f;
     if (c < n) {
-      const int64_t row = a.rowmap[c];
+      const int64_t row = rowmap[c];
       const int64_t at = (row << lkp) + (k & (a.kp - 1));
       idx = a.topk ? a.tgt_idx0[at] : (int)a.labels[row];
       q = a.topk ? a.tgt_q0[at] : 1.f;
@@ -258,7 +288,7 @@ __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, i
   }
   if (backward && blockIdx.y == 0 && t < 64) {
     const bool real = c0 + t < n;
-    const int64_t row = real ? a.rowmap[c0 + t] : 0;
+    const int64_t row = real ? rowmap[c0 + t] : 0;
     a.g[c0 + t] = real && common_scale(a, n) != 0.f ? a.row_weight ? a.row_weight[row] : 1.f : 0.f;
     if (from_lse) a.lse2[c0 + t] = real ? a.lse[row] * LOG2E : 0.f;
   }
@@ -289,7 +319,7 @@ __global__ __launch_bounds__(256) void transpose_kernel(const bf16_t* src, int64
 
 // (distillation) sum_k q_k (log q_k - z_k / T) of a compact row: 16 lanes per entry, the entries' rows of weight gathered.
 // In log2 units, as `finish` has them.  A row with 16 entries or more has four waves: what it takes is the gathers' latency, and one wave
-// after the other through 100 entries took 61 us for 1000 rows, four waves TL_US.
+// after the other through 100 entries took 61 us for 1000 rows, four waves 25.
 constexpr int target_waves(int kp) { return kp >= 16 ? 4 : 1; }
 __global__ __launch_bounds__(256) void target_logits_kernel(LossArgs a) {
   __shared__ float s_sum[4];
@@ -580,14 +610,22 @@ __device__ __forceinline__ float finish_row(const LossArgs& a, int wgs, int64_t 
   }
   const int gs = g0 * O.tiles, ge = gs + (O.tiles << lw);
   float m = -3.0e38f, s = 0.f;
-  for (int w = lane; w < wgs; w += 64) {      // the workgroups that had this row block: they have a pair of its group
-    const int xcd = w >> lslots, q = O.units >> 3, r = O.units & 7;
-    const int base = xcd * q + min(xcd, r), lo = max(gs, base), hi = min(ge, base + q + (xcd < r ? 1 : 0));
-    const int t = lo + ((base + (w & (O.slots - 1)) - lo) & (O.slots - 1));
-    if (t < hi && ((t - gs) & ((1 << lw) - 1)) == rb - g0) {
-      const float2 o = a.part[(int64_t)(group * wgs + w) * C::BM + c % C::BM];
-      const float nm = fmaxf(m, o.x);
-      s = s * __builtin_amdgcn_exp2f(m - nm) + o.y * __builtin_amdgcn_exp2f(o.x - nm);
+  for (int w0 = lane; w0 < wgs; w0 += 256) {      // the workgroups that had this row block: they have a pair of its group
+    float2 o[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {                  // four loads on their way together
+      const int w = w0 + u * 64;
+      const int xcd = w >> lslots, q = O.units >> 3, r = O.units & 7;
+      const int base = xcd * q + min(xcd, r), lo = max(gs, base), hi = min(ge, base + q + (xcd < r ? 1 : 0));
+      const int t = lo + ((base + (w & (O.slots - 1)) - lo) & (O.slots - 1));
+      const bool had = w < wgs && t < hi && ((t - gs) & ((1 << lw) - 1)) == rb - g0;
+      o[u] = make_float2(-3.0e38f, 0.f);
+      if (had) o[u] = a.part[(int64_t)(group * wgs + w) * C::BM + c % C::BM];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float nm = fmaxf(m, o[u].x);
+      s = s * __builtin_amdgcn_exp2f(m - nm) + o[u].y * __builtin_amdgcn_exp2f(o[u].x - nm);
       m = nm;
     }
   }
@@ -609,6 +647,9 @@ __device__ __forceinline__ float finish_row(const LossArgs& a, int wgs, int64_t 
   return loss;
 }
 
+__device__ __forceinline__ float reduced(const LossArgs& a, double sum) {
+  return (float)(a.reduction == CACO_REDUCE_MEAN ? sum / (double)*a.count : sum);      // no row counts: 0 / 0, as torch has it
+}
 // 16 rows to a workgroup.  The sum or mean of the (weighted) row losses: every workgroup leaves its own in `sums`, the last one to arrive
 // adds them in a fixed order.  What passes from one workgroup to another goes past the XCDs' L2s (agent scope), and a workgroup
 // counts itself only after its sum has arrived.
@@ -626,6 +667,13 @@ __global__ __launch_bounds__(1024) void finish_kernel(LossArgs a, int wgs) {
   if (!a.loss) return;
   if (lane == 0) s_sum[wave] = sum;
   __syncthreads();
+  if (gridDim.x == 1) {
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < 16; ++w) sum += s_sum[w];
+      *a.loss = reduced(a, sum);
+    }
+    return;
+  }
   if (threadIdx.x == 0) {
     for (int w = 1; w < 16; ++w) sum += s_sum[w];
     vg_agent_store(a.sums + blockIdx.x, sum);
@@ -642,7 +690,7 @@ __global__ __launch_bounds__(1024) void finish_kernel(LossArgs a, int wgs) {
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < 16; ++w) sum += s_sum[w];
-    *a.loss = (float)(a.reduction == CACO_REDUCE_MEAN ? sum / (double)*a.count : sum);      // no row counts: 0 / 0, as torch has it
+    *a.loss = reduced(a, sum);
   }
 }
 
@@ -996,7 +1044,7 @@ struct Plan {
   int hp, kp;
   int64_t piece;
   bool small;
-  int64_t o_count, o_sums, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_hct, o_part, o_zt, o_lse2, o_g, o_db64, o_dl, o_dlt, o_wt, o_slab, o_dbp;
+  int64_t o_count, o_sums, o_some, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_hct, o_part, o_zt, o_lse2, o_g, o_db64, o_dl, o_dlt, o_wt, o_slab, o_dbp;
   int64_t take(int64_t n) {
     const int64_t at = bytes;
     bytes += up(n, 256);
@@ -1012,6 +1060,7 @@ struct Plan {
     const int bm = small ? Small::BM : Big::BM;
     o_count = take(12);                                        // the largest weight, `arrived`
     o_sums = take(npad / 16 * 8);
+    o_some = topk ? take(npad * 4) : 0;
     o_rowmap = take(npad * 4);
     o_inv = take(npad * 4);
     o_ti0 = topk ? take(npad * kp * 4) : 0;
@@ -1070,8 +1119,9 @@ int run_loss(LossArgs& a, const Plan& P, int what, int cus, hipStream_t st) {
   const int wgs = P.small ? 2 * cus : cus;
   const bool fwd = what & CACO_LOSS_FORWARD, bwd = what & CACO_LOSS_BACKWARD;
   if (a.topk && a.rows) CACO_TRY_RC(launch("loss targets", targets_kernel, rows4, 256, 0, st, a));
-  CACO_TRY_RC(launch("loss compact", compact_kernel, dim3(1), 1024, 0, st, a));
-  CACO_TRY_RC(launch("loss gather", gather_kernel, dim3((unsigned)(P.npad / 64), a.hp / 64), 256, 0, st, a, (int)bwd, (int)!fwd));
+  const bool few = a.rows <= FEW_ROWS;
+  if (!few) CACO_TRY_RC(launch("loss compact", compact_kernel, dim3(1), 1024, 0, st, a));
+  CACO_TRY_RC(launch("loss gather", few ? gather_kernel<true> : gather_kernel<false>, dim3((unsigned)(P.npad / 64), a.hp / 64), 256, 0, st, a, (int)bwd, (int)!fwd));
   if (a.topk) CACO_TRY_RC(launch("loss target logits", target_logits_kernel, target_waves(a.kp) == 4 ? dim3((unsigned)P.npad) : pad4, 256, 0, st, a));
   if (fwd) {
     CACO_TRY_RC(launch("loss lse", lse_kernel<C>, dim3(wgs), C::THREADS, C::SMEM_WFAR, st, a));
@@ -1157,7 +1207,7 @@ int linear_loss(const LinearLoss& c, hipStream_t st) {
   a.row_loss = c.row_loss; a.lse = c.lse; a.loss = c.loss;
   a.dh = bwd ? c.d_hidden : nullptr; a.ld_dh = c.ld_dh; a.dw = bwd ? c.d_weight : nullptr; a.ld_dw = c.ld_dw; a.db = bwd ? c.d_bias : nullptr;
   char* w = reinterpret_cast<char*>(c.ws);
-  a.count = (int*)(w + P.o_count); a.rowmap = (int*)(w + P.o_rowmap); a.inv = (int*)(w + P.o_inv);
+  a.count = (int*)(w + P.o_count); a.some = (int*)(w + P.o_some); a.rowmap = (int*)(w + P.o_rowmap); a.inv = (int*)(w + P.o_inv);
   a.tgt_idx0 = (int*)(w + P.o_ti0); a.tgt_q0 = (float*)(w + P.o_tq0); a.tgt_idx = (int*)(w + P.o_ti); a.tgt_q = (float*)(w + P.o_tq);
   a.hc = (bf16_t*)(w + P.o_hc); a.hct = (bf16_t*)(w + P.o_hct); a.part = (float2*)(w + P.o_part); a.zt = (float*)(w + P.o_zt); a.tgt_z = (float*)(w + P.o_tz); a.lse2 = (float*)(w + P.o_lse2); a.g = (float*)(w + P.o_g);
   a.dl = (bf16_t*)(w + P.o_dl); a.dlt = (bf16_t*)(w + P.o_dlt); a.wt = P.o_wt >= 0 && c.d_hidden ? (bf16_t*)(w + P.o_wt) : nullptr; a.slab = (float*)(w + P.o_slab); a.dbp = (float*)(w + P.o_dbp); a.vpad = P.vpad;
