@@ -306,7 +306,7 @@ __device__ __forceinline__ void attention_body(const bf16_t* __restrict__ qp_, i
         }
         const float m_use = (m_run[x] == -INFINITY) ? 0.f : m_run[x];
         const float neg = -m_use * scale_log2;
-        // packed fp32 math (v_pk_fma_f32 / v_pk_add_f32 work on register pairs) and four independent partial sums
+        // register pairs and four independent partial sums (the build keeps packed fp32 instructions off: two scalar ones per pair)
         typedef float f32x2 __attribute__((ext_vector_type(2)));
         const f32x2 sc2 = {scale_log2, scale_log2}, neg2 = {neg, neg};
         f32x2 ps2[2] = {{0.f, 0.f}, {0.f, 0.f}};
@@ -354,7 +354,7 @@ __device__ __forceinline__ void attention_body(const bf16_t* __restrict__ qp_, i
   // (1) the lane's staging address is re-derived here from an opaque copy of the lane id instead of `lane & 31` being carried
   // from the prologue - at 256 VGPRs the two-block kernel spilled exactly that register around its tile loop (8 bytes of scratch;
   // the thread id it derives from is live through the loop anyway); (2) the
-  // normalisation and bf16 conversion work on register pairs (v_pk_mul_f32 + v_cvt_pk_bf16_f32): the scalar form below compiles
+  // normalisation and bf16 conversion work on register pairs (v_cvt_pk_bf16_f32): the scalar form below compiles
   // to ~150 surplus v_perm / v_alignbit / v_mov per wave around the conversions (profiles/r4_cpu/epilogue_budget.txt).
   int lane_e = lane;
 #ifndef WAVESIM

@@ -41,7 +41,8 @@ constexpr int MAX_CU = 256;
 constexpr int WT_ROWS = 2048;
 
 typedef VgTile<8, 4, 2, 4> Big;      // 256 x 256, one workgroup per CU
-typedef VgTile<4, 2, 1, 4> Small;    // 64 x 128, two per CU: 64 tokens or fewer, where a call reads the weights and does little else
+typedef VgTile<4, 2, 1, 4> Small;    // 64 x 128, two per CU: 64 tokens or fewer, where a call reads the weights and
+                                     // does little else (lse of 768 x 50265 for one token: 18 us, 4.3 TB/s; with Big 30)
 
 // what the kernels share; device pointers into the caller's tensors or the workspace
 struct LossArgs {

@@ -56,9 +56,8 @@ struct __attribute__((aligned(16))) MelSmem {
 constexpr int TP = NMEL + 16;  // log-mel tile pitch
 static_assert(SPAN % 4 == 0 && SPAN >= FPB * TP, "sample span is float4-copyable and holds the log-mel tile");
 
-// Complex numbers are native 2-vectors so that every complex add / multiply maps onto the packed fp32 VALU ops
-// (v_pk_add_f32, v_pk_mul_f32, v_pk_fma_f32: two floats per lane per issue slot); the swaps and sign flips of conj and
-// multiply-by-i fold into the op_sel / neg modifiers of those instructions.
+// Complex numbers are native 2-vectors.  The build keeps the packed fp32 instructions off, so an add or a multiply is one scalar
+// instruction per part; sign flips fold into their neg modifiers.
 __device__ __forceinline__ c32 cmul(c32 a, c32 b) {   // (a.x b.x - a.y b.y, a.x b.y + a.y b.x)
   const c32 bs = {-b.y, b.x};
   return a.xx * b + a.yy * bs;
