@@ -157,6 +157,8 @@ class _LinearLoss(torch.autograd.Function):
         hidden, weight, bias = ctx.saved_tensors[:3]
         head = ctx.head
         with torch.cuda.device(head.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"{head.what}: the autograd form cannot be captured into a graph; capture {head.what}_with_grad")
             new = lambda n, t: torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and ctx.needs_input_grad[n] else None
             dh, dw, db = new(0, hidden), new(1, weight), new(2, bias)
             grad = grad.to(torch.float32).contiguous()

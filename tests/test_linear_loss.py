@@ -501,6 +501,18 @@ def test_autograd_refuses_capture():
 
 
 @pytest.mark.gpu
+def test_a_backward_pass_refuses_capture(monkeypatch):
+    """The forward pass ran before the capture; nothing is captured here, the stream only says so."""
+    from cacophony_amd import losses
+    d = dev(make(20, 150, 64, seed=42))
+    h = d["h"].clone().requires_grad_()
+    loss = losses.linear_cross_entropy(h, d["w"], d["y"], d["b"])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        loss.backward()
+
+
+@pytest.mark.gpu
 def test_calls_on_two_streams_at_once():
     xs = [dev(make(300, 2000, 128, topk=k, seed=30 + k)) for k in (0, 5)]
     want = [with_grad(x) for x in xs]
