@@ -41,8 +41,10 @@ constexpr int MAX_CU = 256;
 constexpr int WT_ROWS = 2048;
 
 typedef VgTile<8, 4, 2, 4> Big;      // 256 x 256, one workgroup per CU
-typedef VgTile<4, 2, 1, 4> Small;    // 64 x 128, two per CU: 64 tokens or fewer, where a call reads the weights and
-                                     // does little else (lse of 768 x 50265 for one token: 18 us, 4.3 TB/s; with Big 30)
+typedef VgTile<4, 2, 1, 4> Small;    // 64 x 128, two per CU: for calls that read the weights and do little else
+// Up to this many rows take Small.  768 x 50265: lse for one token 18 us (4.3 TB/s), with Big 30; a call with gradients for 65 / 128 rows 135 / 143 us, with
+// Big 143 / 150 (520 x 32007: 106 / 110, with Big 121 / 125).  From 129 rows on Big is as fast or faster (149 rows: 154 us, with Small 173).
+constexpr int SMALL_ROWS = 128;
 
 // what the kernels share; device pointers into the caller's tensors or the workspace
 struct LossArgs {
@@ -1057,7 +1059,7 @@ struct Plan {
     hp = (int)up(dim, VG_K);
     kp = 1;
     while (kp < topk) kp *= 2;
-    small = rows <= Small::BM;
+    small = rows <= SMALL_ROWS;
     const int bm = small ? Small::BM : Big::BM;
     o_count = take(12);                                        // the largest weight, `arrived`
     o_sums = take(npad / 16 * 8);
