@@ -979,56 +979,76 @@ __device__ __forceinline__ void dbias(const LossArgs& a, int v, int bm, int wm) 
 
 // What is left to add up, in order, once the pieces are through.  The first `joins` workgroups: d hidden's parts, rounded once, 8 compact rows x
 // 256 of dim each, and zeros for those of the caller's rows with the same numbers that do not count.  The others: d bias, 256 words each.
+// G = 8: one row to a workgroup, every eighth part to 32 threads, these eight sums added in order.  With one block of rows a tile has up to 8 * 32
+// parts and there are few rows to share them out by.
+template <int G>
 __global__ __launch_bounds__(256) void close_kernel(LossArgs a, int wgs, int joins, int bm, int wm) {
   if ((int)blockIdx.x >= joins) {
     dbias(a, ((int)blockIdx.x - joins) * 256 + threadIdx.x, bm, wm);
     return;
   }
   const int cbs = (a.dim + 255) / 256, by = (int)blockIdx.x % cbs;
-  __shared__ int s_place[8][MAX_CU / 8 + 1], s_parts[8], s_list[8 * (MAX_CU / 8 + 1)];
-  const int n = *a.count, t = threadIdx.x;
-  const int64_t c0 = (int64_t)((int)blockIdx.x / cbs) * 8, c = c0 + t / 32;
+  __shared__ int s_parts[4], s_list[MAX_CU];
+  __shared__ f32x4 s_sum[G == 1 ? 1 : 256][2];
+  const int n = *a.count, t = threadIdx.x, grp = G == 1 ? 0 : t / 32;
+  const int64_t c0 = (int64_t)((int)blockIdx.x / cbs) * (8 / G), c = G == 1 ? c0 + t / 32 : c0;
   const int x = by * 256 + t % 32 * 8;
-  if (c < a.rows && x < a.dim && a.inv[c] < 0) *reinterpret_cast<bf16x8*>(a.dh + c * a.ld_dh + x) = bf16x8{};
+  if (grp == 0 && c < a.rows && x < a.dim && a.inv[c] < 0) *reinterpret_cast<bf16x8*>(a.dh + c * a.ld_dh + x) = bf16x8{};
   if (c0 >= n) return;
-  // where the parts of this output tile are: one thread per XCD
-  if (t < 8) {
-    const Share S(a, n, wgs, t);
-    const int o = (int)(c0 / 256) * S.cb + by, i = o - S.t0 - S.whole * S.slots;      // the tile's place in the list
-    int parts = 0;
-    if (o >= S.t0 && i < S.rest) {
-      if (i < 0) s_place[t][parts++] = (int)S.slab_whole(o);
-      else
-        for (int s = 0; s < S.slots && S.first(s) < (i + 1) * S.nkx; ++s)
-          if (S.first(s + 1) > i * S.nkx && S.first(s + 1) > S.first(s)) s_place[t][parts++] = (int)S.slab_list(t, i, s);
+  // where the parts of this output tile are: a thread per workgroup of `grads`, 32 to an XCD; the list in their order
+  static_assert(MAX_CU == 256, "a thread per workgroup");
+  int place = -1;
+  {
+    const Share S(a, n, wgs, t >> 5);
+    const int o = (int)(c0 / 256) * S.cb + by, i = o - S.t0 - S.whole * S.slots, s = t & 31;      // i: the tile's place in the list
+    if (o >= S.t0 && i < S.rest && s < S.slots) {
+      if (i < 0) {
+        if (s == 0) place = (int)S.slab_whole(o);
+      } else {
+        const int f0 = S.first(s), f1 = S.first(s + 1);
+        if (f0 < (i + 1) * S.nkx && f1 > i * S.nkx && f1 > f0) place = (int)S.slab_list(t >> 5, i, s);
+      }
     }
-    s_parts[t] = parts;
   }
+  const unsigned long long mask = __ballot(place >= 0);
+  if ((t & 63) == 0) s_parts[t >> 6] = __builtin_popcountll(mask);
   __syncthreads();
-  int parts = 0;
-  for (int xcd = 0; xcd < 8; ++xcd) {
-    if (t < s_parts[xcd]) s_list[parts + t] = s_place[xcd][t];
-    parts += s_parts[xcd];
+  int parts = 0, at = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < t >> 6) at += s_parts[w];
+    parts += s_parts[w];
   }
+  if (place >= 0) s_list[at + __builtin_popcountll(mask & ((1ull << (t & 63)) - 1))] = place;
   __syncthreads();
-  if (x >= a.dim || c >= n) return;
+  if (G == 1 && (x >= a.dim || c >= n)) return;
   f32x4 v[2] = {};
   const float* p = a.slab + (c % 256) * 256 + t % 32 * 8;
-  int k = 0;
-  for (; k + 8 <= parts; k += 8) {      // a tile of the list has up to 8 * 32 parts: their loads must not wait for one another
+  int k = grp;
+  for (; k + 7 * G < parts; k += 8 * G) {      // their loads must not wait for one another
     f32x4 u[8][2];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) u[j][h] = *reinterpret_cast<const f32x4*>(p + (int64_t)s_list[k + j] * 65536 + h * 4);
+      for (int h = 0; h < 2; ++h) u[j][h] = *reinterpret_cast<const f32x4*>(p + (int64_t)s_list[k + j * G] * 65536 + h * 4);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int h = 0; h < 2; ++h) v[h] += u[j][h];
   }
-  for (; k < parts; ++k)
+  for (; k < parts; k += G)
 #pragma unroll
     for (int h = 0; h < 2; ++h) v[h] += *reinterpret_cast<const f32x4*>(p + (int64_t)s_list[k] * 65536 + h * 4);
+  if (G != 1) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) s_sum[t][h] = v[h];
+    __syncthreads();
+    if (grp || x >= a.dim) return;
+#pragma unroll
+    for (int g = 1; g < G; ++g)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) v[h] += s_sum[g * 32 + t][h];
+  }
   const float scale = common_scale(a, n);
   bf16x8 o8;
 #pragma unroll
@@ -1107,6 +1127,10 @@ int64_t piece_for(int64_t rows, int vocab, int64_t budget) {
   return up((all + pieces - 1) / pieces, 256);
 }
 
+// Up to this many rows `close` takes one row to a workgroup.  768 x 50265, us for 37 / 256 / 1000 / 2000 rows: 5.4 / 12.7 / 17.1 / 22.5; with eight rows
+// 15.4 / 18.8 / 20.2 / 21.5.
+constexpr int ONE_ROW = 1024;
+
 template <typename K, typename... A>
 int launch(const char* what, K kern, dim3 grid, int threads, int lds, hipStream_t st, A... args) {
   int num_cu = 0;
@@ -1140,8 +1164,10 @@ int run_loss(LossArgs& a, const Plan& P, int what, int cus, hipStream_t st) {
                          (int64_t)(a.vocab - a.v0), a.dim, a.wt, (int64_t)a.piece));
     if (a.dh || a.dw) CACO_TRY_RC(launch("loss grads", a.wt ? grads_kernel<true> : grads_kernel<false>, dim3(cus), Big::THREADS, Big::SMEM_XFAR, st, a));
   }
-  const int64_t joins = a.dh ? (a.rows + 7) / 8 * ((a.dim + 255) / 256) : 0, words = a.db ? (a.vocab + 255) / 256 : 0;
-  if (joins + words) CACO_TRY_RC(launch("loss close", close_kernel, dim3((unsigned)(joins + words)), 256, 0, st, a, cus, (int)joins, (int)C::BM, (int)C::WM));
+  const bool one = a.rows <= ONE_ROW;
+  const int64_t joins = a.dh ? (one ? a.rows : (a.rows + 7) / 8) * ((a.dim + 255) / 256) : 0, words = a.db ? (a.vocab + 255) / 256 : 0;
+  if (joins + words)
+    CACO_TRY_RC(launch("loss close", one ? close_kernel<8> : close_kernel<1>, dim3((unsigned)(joins + words)), 256, 0, st, a, cus, (int)joins, (int)C::BM, (int)C::WM));
   return CACO_OK;
 }
 
