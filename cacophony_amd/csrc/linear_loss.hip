@@ -23,6 +23,7 @@
 //   targets2     (distillation) the entries of the teacher's tokens, from the logits that the loss was taken from
 //   grads        d weight's tiles (sums over the tokens, complete) and d hidden (sums over the vocabulary, cut into one run per
 //                workgroup that makes up for the uneven number of d weight's tiles; partial sums are kept in fp32)
+//   join weight  (few of d weight's tiles and many tokens) adds d weight's runs of tokens in order
 //   close        adds d hidden's partial sums and d bias's column sums in order
 // Nothing is accumulated in an order that can change: equal calls give equal bits.
 #define CACO_WAVE_SYNC_FENCE
@@ -45,6 +46,10 @@ typedef VgTile<4, 2, 1, 4> Small;    // 64 x 128, two per CU: for calls that rea
 // Up to this many rows take Small.  768 x 50265: lse for one token 18 us (4.3 TB/s), with Big 30; a call with gradients for 65 / 128 rows 135 / 143 us, with
 // Big 143 / 150 (520 x 32007: 106 / 110, with Big 121 / 125).  From 129 rows on Big is as fast or faster (149 rows: 154 us, with Small 173).
 constexpr int SMALL_ROWS = 128;
+// ... and so do calls that would have at most this many of Big's tiles, which would leave half the CUs idle.  Calls with gradients, us, rows x
+// vocabulary x dim: 24 tiles (700 x 2000 x 2048) 94, with Big 147; 48 (300 x 6000 x 512) 63, 84; 118 (300 x 15000 x 512) 102, 107; 160 (1000 x 10000 x 512)
+// 119, 114; 236 (300 x 30000 x 1000) 208, 197.
+constexpr int SMALL_TILES = 128;
 
 // what the kernels share; device pointers into the caller's tensors or the workspace
 struct LossArgs {
@@ -85,6 +90,7 @@ struct LossArgs {
   // other's way, either alone is as fast.)
   bf16_t *dl, *dlt;
   bf16_t* wt;                        // the piece's weights transposed [dim, piece], zeros past the vocabulary; or null
+  float* wslab; int lw;              // d weight in 2^lw runs of tokens: partial sums [piece's tile][run][256][256]
   float* slab;                       // d hidden's partial sums [output tile + workgroup][256][256]
   float* dbp; int64_t vpad;          // column sums of d logits [row halves, vpad = vocabulary rounded up to 256]
   int piece, v0;                     // columns of the piece, its first column
@@ -836,8 +842,8 @@ __global__ __launch_bounds__(256) void targets2_kernel(LossArgs a) {
 // part, so the places are distinct).
 struct Share {
   int rb, cb, tiles, nk, ks;       // d hidden: row blocks, column blocks, output tiles, K-tiles of one, slices
-  int nkw, slots;                  // d weight: K-tiles of a tile; workgroups of an XCD
-  int wcnt, wbase;                 // this XCD's d weight tiles, the first
+  int nka, nkw, slots;             // d weight: K-tiles of a tile, at most of one of its runs; workgroups of an XCD
+  int wcnt, wbase;                 // this XCD's d weight runs, the first
   int slice, k0, nkx;              // its slice, the slice's first K-tile and length
   int t0, whole, rest;             // its output tiles: the first, whole ones per workgroup, tiles in the list
   int more, few, many;             // workgroups with a d weight tile more; K-tiles of the list for these and for the others
@@ -849,8 +855,9 @@ struct Share {
     cb = (a.dim + 255) / 256;
     tiles = rb * cb;
     nk = a.piece / VG_K;
-    nkw = (n + VG_K - 1) / VG_K;
-    const int wt = a.dw ? a.piece / 256 * cb : 0;
+    nka = (n + VG_K - 1) / VG_K;
+    nkw = (nka + (1 << a.lw) - 1) >> a.lw;
+    const int wt = a.dw ? (a.piece / 256 * cb) << a.lw : 0;
     wcnt = (wt >> 3) + (xcd < (wt & 7) ? 1 : 0);
     wbase = xcd * (wt >> 3) + min(xcd, wt & 7);
     int lks = 0;
@@ -896,20 +903,32 @@ __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
   if (slot < S.wcnt)
     vg_run<C, false, false, false, false, false>(
         (S.wcnt - slot + S.slots - 1) / S.slots, smem,
-        [&](int, int& k0, int& k1) { k0 = 0; k1 = S.nkw; },
-        [&](int i) {
-          const int tm = (S.wbase + slot + i * S.slots) / S.cb;
-          return VgOperand{a.dlt + (int64_t)tm * 65536, 256, C::BM, S.nkw * VG_K, (int64_t)a.piece * 256};
+        [&](int i, int& k0, int& k1) {
+          const int run = (S.wbase + slot + i * S.slots) & ((1 << a.lw) - 1);
+          k0 = (run * S.nka) >> a.lw;
+          k1 = ((run + 1) * S.nka) >> a.lw;
         },
         [&](int i) {
-          const int c = (S.wbase + slot + i * S.slots) % S.cb * C::BN;
-          return VgOperand{a.hct + c * a.npad, a.npad, a.hp - c, S.nkw * VG_K, 0};
+          const int tm = ((S.wbase + slot + i * S.slots) >> a.lw) / S.cb;
+          return VgOperand{a.dlt + (int64_t)tm * 65536, 256, C::BM, S.nka * VG_K, (int64_t)a.piece * 256};
+        },
+        [&](int i) {
+          const int c = ((S.wbase + slot + i * S.slots) >> a.lw) % S.cb * C::BN;
+          return VgOperand{a.hct + c * a.npad, a.npad, a.hp - c, S.nka * VG_K, 0};
         },
         VgNoWords{}, VgZero{},
         [&](int i, f32x4 (&acc)[C::MI][C::NI], char* free_slot) {
           const int lane = vg_lane(), l16 = lane & 15, lq = lane >> 4;
           char* slab = free_slot + wave * C::SLAB;
-          const int t = S.wbase + slot + i * S.slots, tn = t % S.cb, tm = t / S.cb;
+          const int u = S.wbase + slot + i * S.slots, t = u >> a.lw, tn = t % S.cb, tm = t / S.cb;
+          if (a.lw) {
+            float* d = a.wslab + (int64_t)u * C::BM * C::BN + (wm * 16 * C::MI + l16) * C::BN + wn * 16 * C::NI + lq * 4;
+#pragma unroll
+            for (int q = 0; q < C::MI; ++q)
+#pragma unroll
+              for (int j = 0; j < C::NI; ++j) *reinterpret_cast<f32x4*>(d + q * 16 * C::BN + j * 16) = acc[q][j];
+            return;
+          }
           const int v0 = a.v0 + tm * C::BM + wm * 16 * C::MI, c0 = tn * C::BN + wn * 16 * C::NI;
 #pragma unroll
           for (int q = 0; q < C::MI; ++q) {
@@ -965,6 +984,24 @@ template <bool WT>
 __global__ __launch_bounds__(Big::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void grads_kernel(LossArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   grads_body<WT>(a, smem);
+}
+
+// d weight from its runs of tokens, in order: 8 rows of a tile to a workgroup
+__global__ __launch_bounds__(256) void join_weight_kernel(LossArgs a) {
+  const int cb = (a.dim + 255) / 256, tile = blockIdx.x >> 5, row = (blockIdx.x & 31) * 8 + threadIdx.x / 32, col = threadIdx.x % 32 * 8;
+  const int v = a.v0 + tile / cb * 256 + row, x = tile % cb * 256 + col;
+  if (v >= a.vocab || x >= a.dim) return;
+  const float* p = a.wslab + ((int64_t)tile << a.lw) * 65536 + row * 256 + col;
+  f32x4 s[2] = {};
+#pragma unroll 4
+  for (int r = 0; r < 1 << a.lw; ++r)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) s[h] += *reinterpret_cast<const f32x4*>(p + (int64_t)r * 65536 + h * 4);
+  const float scale = common_scale(a, *a.count);
+  bf16x8 o;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = (bf16_t)(s[e / 4][e % 4] * scale);
+  *reinterpret_cast<bf16x8*>(a.dw + (int64_t)v * a.ld_dw + x) = o;
 }
 
 __device__ __forceinline__ void dbias(const LossArgs& a, int v, int bm, int wm) {
@@ -1067,7 +1104,8 @@ struct Plan {
   int hp, kp;
   int64_t piece;
   bool small;
-  int64_t o_count, o_sums, o_some, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_hct, o_part, o_zt, o_lse2, o_g, o_db64, o_dl, o_dlt, o_wt, o_slab, o_dbp;
+  int lw = 0;
+  int64_t o_wslab = 0, o_count, o_sums, o_some, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_hct, o_part, o_zt, o_lse2, o_g, o_db64, o_dl, o_dlt, o_wt, o_slab, o_dbp;
   int64_t take(int64_t n) {
     const int64_t at = bytes;
     bytes += up(n, 256);
@@ -1079,7 +1117,7 @@ struct Plan {
     hp = (int)up(dim, VG_K);
     kp = 1;
     while (kp < topk) kp *= 2;
-    small = rows <= SMALL_ROWS;
+    small = rows <= SMALL_ROWS || npad / 256 * ((vocab + 255) / 256) <= SMALL_TILES;
     const int bm = small ? Small::BM : Big::BM;
     o_count = take(12);                                        // the largest weight, `arrived`
     o_sums = take(npad / 16 * 8);
@@ -1106,6 +1144,12 @@ struct Plan {
       o_dlt = take(npad * piece * 2);
       o_wt = rows >= WT_ROWS ? take((int64_t)dim * piece * 2) : -1;
       o_slab = take(Share::slabs(npad / 256 * ((dim + 255) / 256), MAX_CU / 8) * 65536 * 4);
+      // A small vocabulary has few tiles of d weight, and many tokens make them long: they are cut into runs of 8 K-tiles or more as long as
+      // there are CUs for them, from 1536 tokens on.  Calls with gradients, us, rows x vocabulary x dim: 1000 x 6000 x 512 103, uncut 96; 2000 x 2000 x 1000
+      // 125, 143; 8192 x 300 x 2000 196, 294; 8192 x 1000 x 64 119, 233.  (The whole vocabulary's tiles count: the size is then the same for every piece.)
+      const int64_t wtiles = (int64_t)(vocab + 255) / 256 * ((dim + 255) / 256);
+      while (npad >= 1536 && (wtiles << (lw + 1)) <= MAX_CU && (npad / VG_K >> (lw + 1)) >= 8) ++lw;
+      if (lw) o_wslab = take((wtiles << lw) * 65536 * 4);
       vpad = up(vocab, 256);
       o_dbp = take(npad / bm * (small ? Small::WM : Big::WM) * vpad * 4);
     }
@@ -1163,6 +1207,7 @@ int run_loss(LossArgs& a, const Plan& P, int what, int cus, hipStream_t st) {
       CACO_TRY_RC(launch("loss weight transpose", transpose_kernel, dim3(a.piece / 64, (a.dim + 63) / 64), 256, 0, st, a.weight + a.v0 * a.ld_w, a.ld_w,
                          (int64_t)(a.vocab - a.v0), a.dim, a.wt, (int64_t)a.piece));
     if (a.dh || a.dw) CACO_TRY_RC(launch("loss grads", a.wt ? grads_kernel<true> : grads_kernel<false>, dim3(cus), Big::THREADS, Big::SMEM_XFAR, st, a));
+    if (a.dw && a.lw) CACO_TRY_RC(launch("loss join weight", join_weight_kernel, dim3((unsigned)(a.piece / 256 * ((a.dim + 255) / 256) * 32)), 256, 0, st, a));
   }
   const bool one = a.rows <= ONE_ROW;
   const int64_t joins = a.dh ? (one ? a.rows : (a.rows + 7) / 8) * ((a.dim + 255) / 256) : 0, words = a.db ? (a.vocab + 255) / 256 : 0;
@@ -1239,7 +1284,7 @@ int linear_loss(const LinearLoss& c, hipStream_t st) {
   a.count = (int*)(w + P.o_count); a.some = (int*)(w + P.o_some); a.rowmap = (int*)(w + P.o_rowmap); a.inv = (int*)(w + P.o_inv);
   a.tgt_idx0 = (int*)(w + P.o_ti0); a.tgt_q0 = (float*)(w + P.o_tq0); a.tgt_idx = (int*)(w + P.o_ti); a.tgt_q = (float*)(w + P.o_tq);
   a.hc = (bf16_t*)(w + P.o_hc); a.hct = (bf16_t*)(w + P.o_hct); a.part = (float2*)(w + P.o_part); a.zt = (float*)(w + P.o_zt); a.tgt_z = (float*)(w + P.o_tz); a.lse2 = (float*)(w + P.o_lse2); a.g = (float*)(w + P.o_g);
-  a.dl = (bf16_t*)(w + P.o_dl); a.dlt = (bf16_t*)(w + P.o_dlt); a.wt = P.o_wt >= 0 && c.d_hidden ? (bf16_t*)(w + P.o_wt) : nullptr; a.slab = (float*)(w + P.o_slab); a.dbp = (float*)(w + P.o_dbp); a.vpad = P.vpad;
+  a.dl = (bf16_t*)(w + P.o_dl); a.dlt = (bf16_t*)(w + P.o_dlt); a.wt = P.o_wt >= 0 && c.d_hidden ? (bf16_t*)(w + P.o_wt) : nullptr; a.slab = (float*)(w + P.o_slab); a.wslab = (float*)(w + P.o_wslab); a.lw = P.lw; a.dbp = (float*)(w + P.o_dbp); a.vpad = P.vpad;
   a.wmax = (float*)(a.count + 1); a.arrived = (unsigned*)(a.count + 2); a.sums = (double*)(w + P.o_sums); a.db64 = (unsigned long long*)(w + P.o_db64);
   a.piece = (int)piece;
   int num_cu = 0;

@@ -115,6 +115,9 @@ def close(got, want, what):
 SHAPES = [
     (1, 1, 8, 0, 1.0, True), (1, 257, 64, 0, 1.0, True), (5, 300, 72, 0, 1.0, False), (64, 256, 128, 0, 1.0, True), (65, 513, 136, 0, 1.0, True),
     (256, 255, 64, 0, 1.0, False), (257, 700, 264, 0, 1.0, True),
+    # more than 128 of the large tiles; d weight in runs of tokens (1500 rows and more, few tiles)
+    (257, 16500, 72, 0, 1.0, True), (130, 33000, 8, 3, 2.0, True), (600, 11100, 136, 0, 1.0, False),
+    (1024, 300, 72, 0, 1.0, True), (1500, 257, 264, 4, 1.0, True), (4100, 40, 8, 0, 1.0, True),
     (1, 40, 64, 1, 1.0, True), (7, 500, 64, 5, 2.0, False), (66, 300, 200, 33, 0.5, True), (130, 600, 72, 128, 4.0, True),
 ]
 
