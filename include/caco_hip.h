@@ -178,7 +178,7 @@ int caco_decoder_forward(caco_model* m, const float* text_hidden_dev, const int6
 
 /* ... and the likelihoods of given tokens instead of the logits: nll_dev fp32 [B, T] = -log softmax(logits[b, t])[targets[b, t]], 0 where
  * targets_dev int64 [B, T] is ignore_index or outside the vocabulary.  The reference has the logits only (caco.py:212-240); scoring 256
- * captions of 32 tokens through them takes 3.2 GB of logits, this call about 0.2 GB of scratch. */
+ * captions of 32 tokens through them takes 3.3 GB for the logits (scratch and output), this call 18 MB in their place. */
 int caco_decoder_score(caco_model* m, const float* text_hidden_dev, const int64_t* text_mask_dev, const float* audio_hidden_dev,
                        const float* audio_mask_dev, const int64_t* targets_dev, int64_t ignore_index, int32_t batch, int32_t seq_text,
                        int32_t seq_audio, float* nll_dev, void* stream);

@@ -129,3 +129,24 @@ def test_models_without_a_decoder_refuse(tiny_state):
         plain.get_caption_nll(torch.zeros(1, 8, 768), torch.ones(1, 8), torch.zeros(1, 4, dtype=torch.long), torch.ones(1, 4))
     with pytest.raises(ValueError, match="use_decoder=True"):
         captioning.score_captions(plain, {}, torch.zeros(1, 4, dtype=torch.long), torch.ones(1, 4))
+
+
+@pytest.mark.gpu
+def test_nll_on_another_stream_and_after_other_work(model, clips):
+    """A side stream has an arena of its own; what ran in it before (the decoder's logits, a larger batch) leaves no trace.  Equal calls give
+    equal bits.  Equal captions in one call have equal hidden states, but their logits' exponentials are shared out over other workgroups:
+    50265 of them added up in parts of at most 197 tiles, 256 words, 8 waves and 512 pairs, each sum off by 2^-24 per addition, below 1000 * 2^-24 =
+    6e-5 of the sum and so in its logarithm."""
+    ab, ah = clips
+    ids, mask = synth.make_captions(2, 20, model.text_config.vocab_size, start=11)
+    want = model.get_caption_nll(ah, ab["audio_mask"], ids, mask)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        model.get_decoder_logits(ah, ab["audio_mask"], ids, mask)
+        many = torch.as_tensor(ids).repeat(20, 1), torch.as_tensor(mask).repeat(20, 1)
+        large = model.get_caption_nll(ah.repeat(20, 1, 1), ab["audio_mask"].repeat(20, 1), *many)
+        got = model.get_caption_nll(ah, ab["audio_mask"], ids, mask)
+    side.synchronize()
+    assert torch.equal(got, want)
+    assert (large[:2] - large[38:]).abs().max() < 1e-4
