@@ -474,6 +474,30 @@ def test_captured_and_replayed_between_eager_calls(topk):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,dim,topk", [(2100, 700, 72, 0), (2100, 300, 264, 100), (40, 20000, 64, 7), (900, 17000, 64, 3)])
+def test_equal_bits_in_pieces_and_in_a_graph(rows, vocab, dim, topk):
+    """d weight in runs of tokens, transposed weights, few words that many teacher entries share; one row to a workgroup at the end."""
+    x, y = (dev(make(rows, vocab, dim, topk=topk, seed=s)) for s in (60, 61))
+    static = {k: v.clone() if torch.is_tensor(v) else v for k, v in x.items()}
+    with_grad(static)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = with_grad(static)
+    for z in (x, y, x):
+        for k, v in static.items():
+            if torch.is_tensor(v):
+                v.copy_(z[k])
+        graph.replay()
+        torch.cuda.synchronize()
+        e = with_grad(z)
+        for a, b in zip(out, e):
+            assert torch.equal(a, b)
+        p = with_grad(z, piece_bytes=1)
+        assert torch.equal(p.d_weight, e.d_weight) and torch.equal(p.d_bias, e.d_bias) and torch.equal(p.row_loss, e.row_loss)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("name", ["h", "w", "b", "y", "teacher", "idx"])
 def test_an_operand_changed_before_the_backward_pass_is_an_error(name):
     from cacophony_amd import losses
