@@ -82,8 +82,8 @@ struct LossArgs {
   float* zt;                         // cross entropy: the label's logit; distillation: sum_k q_k (z_k / T - log q_k), log2 units
   float* tgt_z;                      // distillation: the entries' log2-logits [npad, kp]
   float *lse2, *g;                   // compact: lse in log2 units, the row's weight in the gradients
-  float* wmax;                       // largest |row_weight| of the rows that count
-  unsigned long long* db64;          // distillation: sum of the targets' weights per word, fixed point in units of 2^(e - 38), |g| < 2^e
+  // distillation, d bias: per word the exponent field of the largest |g q| of its entries, and their sum as an integer (see targets2_kernel)
+  unsigned* dbe; unsigned long long* db64;
   // d logits of the piece in blocks of 256 rows x 256 columns, [row block][column block][256][256], once with the columns next to one another
   // (d hidden sums over them) and once with the rows (d weight): both products then read fragments of 16 bytes.  (One copy and
   // transposing reads in one of the products: 2.2 us per K-tile of it instead of 1.6; those reads and the loads into LDS get in each
@@ -166,6 +166,9 @@ __global__ __launch_bounds__(256) void targets_kernel(LossArgs a) {
 // the 256 x 256 block of d logits that holds (row, col)
 __device__ __forceinline__ int64_t dl_block(const LossArgs& a, int64_t row, int col) { return ((row >> 8) * (a.piece >> 8) + (col >> 8)) * 65536; }
 
+// the exponent field: 0 for zero and what lies below the normal numbers, 255 for NaN and the infinities
+__device__ __forceinline__ unsigned float_exponent(float x) { return __float_as_uint(x) >> 23 & 255; }
+
 // does row r count?
 __device__ __forceinline__ bool row_counts(const LossArgs& a, int64_t r) {
   if (a.labels) {
@@ -179,10 +182,8 @@ __device__ __forceinline__ bool row_counts(const LossArgs& a, int64_t r) {
 constexpr int FEW_ROWS = 64;
 
 // One workgroup: every wave counts a run of consecutive rows, 64 at a time; a scan over the waves gives each run its first place.
-// Also the largest |row_weight| of the rows that count.
 __global__ __launch_bounds__(1024) void compact_kernel(LossArgs a) {
   __shared__ int s_n[16];
-  __shared__ float s_max[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t per = (a.rows + 1023) / 1024 * 64;
   const int64_t r0 = min(a.rows, wave * per), r1 = min(a.rows, r0 + per);
@@ -192,25 +193,16 @@ __global__ __launch_bounds__(1024) void compact_kernel(LossArgs a) {
   __syncthreads();
   int at = 0;
   for (int w = 0; w < wave; ++w) at += s_n[w];
-  float wmax = a.row_weight ? 0.f : 1.f;
   for (int64_t r = r0; r < r1; r += 64) {
     const int64_t row = r + lane;
     const bool c = row < r1 && row_counts(a, min(row, r1 - 1));
     const unsigned long long mask = __ballot(c);
     const int place = at + __builtin_popcountll(mask & ((1ull << lane) - 1));
     if (row < r1) a.inv[row] = c ? place : -1;
-    if (c) {
-      a.rowmap[place] = (int)row;
-      if (a.row_weight) wmax = fmaxf(wmax, fabsf(a.row_weight[row]));
-    }
+    if (c) a.rowmap[place] = (int)row;
     at += __builtin_popcountll(mask);
   }
-  wmax = wave_max(wmax);
-  if (lane == 0) s_max[wave] = wmax;
-  __syncthreads();
   if (threadIdx.x == 1023) {
-    for (int w = 0; w < 16; ++w) wmax = fmaxf(wmax, s_max[w]);
-    *a.wmax = wmax;
     *a.count = at;
     *a.arrived = 0;
   }
@@ -245,9 +237,7 @@ __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, i
     if (t < 64 && blockIdx.x == 0 && blockIdx.y == 0) {
       if (r < a.rows) a.inv[r] = c ? place : -1;
       if (c) a.rowmap[place] = r;
-      const float wmax = wave_max(!a.row_weight ? 1.f : c ? fabsf(a.row_weight[r]) : 0.f);
       if (r == 0) {
-        *a.wmax = wmax;
         *a.count = n;
         *a.arrived = 0;
       }
@@ -259,7 +249,10 @@ __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, i
   const int* rowmap = FEW ? s_row : a.rowmap;
   const int h0 = blockIdx.y * 64;
   if (backward && a.db && a.topk)
-    for (int64_t v = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + t; v < a.vocab; v += (int64_t)gridDim.x * gridDim.y * 256) a.db64[v] = 0;
+    for (int64_t v = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + t; v < a.vocab; v += (int64_t)gridDim.x * gridDim.y * 256) {
+      a.db64[v] = 0;
+      a.dbe[v] = 0;
+    }
   if (c0 >= ((int64_t)n + 255) / 256 * 256) return;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -329,6 +322,7 @@ __global__ __launch_bounds__(256) void transpose_kernel(const bf16_t* src, int64
 // (distillation) sum_k q_k (log q_k - z_k / T) of a compact row: 16 lanes per entry, the entries' rows of weight gathered.
 // In log2 units, as `finish` has them.  A row with 16 entries or more has four waves: what it takes is the gathers' latency, and one wave
 // after the other through 100 entries took 61 us for 1000 rows, four waves 25.
+// With d bias, each entry also leaves its exponent with its word.
 constexpr int target_waves(int kp) { return kp >= 16 ? 4 : 1; }
 __global__ __launch_bounds__(256) void target_logits_kernel(LossArgs a) {
   __shared__ float s_sum[4];
@@ -339,6 +333,7 @@ __global__ __launch_bounds__(256) void target_logits_kernel(LossArgs a) {
   float sum = 0.f;
   if (real) {
     const bf16_t* h = a.hc + c * a.hp;
+    const float g = a.db ? a.g[c] : 0.f;
     const int share = a.kp / waves;                       // up to 32 entries of this wave, in steps of four
     const int at = l16 * 4 + grp;                         // lane (step, group) brings that step's entry of the group: all of them at once
     const int64_t first = c * a.kp + part * share;
@@ -364,6 +359,10 @@ __global__ __launch_bounds__(256) void target_logits_kernel(LossArgs a) {
         z *= a.inv_t * LOG2E;
         sum += q * (log2f(q) - z);
         a.tgt_z[first + s * 4 + grp] = z;
+        if (g != 0.f) {
+          const unsigned x = max(float_exponent(g * q), 1u);      // below the normal numbers the units stay the same
+          if (a.dbe[idx] < x) atomicMax(a.dbe + idx, x);          // it only grows: an old value costs an atomic, not an answer
+        }
       }
     }
     sum = wave_sum(sum);
@@ -807,15 +806,10 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
   dlogits_body<C>(a, smem);
 }
 
-// exponent e of the fixed point: every |g| < 2^e (0 where the largest is not finite or is zero)
-__device__ __forceinline__ int fixed_exponent(const LossArgs& a) {
-  const unsigned m = __float_as_uint(*a.wmax);
-  return m == 0 || m >= 0x7f800000u ? 0 : max((int)(m >> 23), 1) - 126;
-}
-
 // (distillation) d logits at the teacher's tokens of the piece: one thread per entry.  The tokens of a row are distinct, so an entry is
-// written by one thread.  Their share of d bias is added as 64-bit integers, whose sum does not depend on the order: an entry is below
-// 2^38 units (q <= 1), the 2^22 rows' sum below 2^62, and a unit is 2^-38 of the largest |g|.
+// written by one thread.  Their share of d bias, g q, is added as 64-bit integers, whose sum does not depend on the order.  A word has units of its
+// own: with E the exponent field of its largest |g q|, that one is below 2^(E - 126) = 2^39 units, the sum of 2^22 rows below 2^61, and what an
+// entry loses is at most 2^-39 of the largest, less than the roundings of a sum in fp32.  E = 255: one of them is not finite, and `dbias` says so.
 __global__ __launch_bounds__(256) void targets2_kernel(LossArgs a) {
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t c = t / a.kp;
@@ -828,8 +822,8 @@ __global__ __launch_bounds__(256) void targets2_kernel(LossArgs a) {
   a.dl[block + (c & 255) * 256 + (v & 255)] = d;
   if (a.dw) a.dlt[block + (v & 255) * 256 + (c & 255)] = d;
   if (!a.db) return;
-  const float x = ldexpf(g * q, 38 - fixed_exponent(a));
-  if (fabsf(x) <= 0x1p38f) atomicAdd(a.db64 + idx, (unsigned long long)(long long)rintf(x));
+  const int E = (int)a.dbe[idx];
+  if (E < 255) atomicAdd(a.db64 + idx, (unsigned long long)(long long)rintf(ldexpf(g * q, 39 + 126 - E)));
 }
 
 // How a piece's gradient work is shared out, XCD by XCD.
@@ -1010,7 +1004,7 @@ __device__ __forceinline__ void dbias(const LossArgs& a, int v, int bm, int wm) 
   float s = 0.f;
 #pragma unroll 8
   for (int p = 0; p < parts; ++p) s += a.dbp[p * a.vpad + v];
-  if (a.topk) s -= (float)ldexp((double)(long long)a.db64[v], fixed_exponent(a) - 38);
+  if (a.topk) s = a.dbe[v] < 255 ? (float)((double)s - ldexp((double)(long long)a.db64[v], (int)a.dbe[v] - 126 - 39)) : NAN;
   a.db[v] = s * common_scale(a, *a.count);
 }
 
@@ -1105,7 +1099,7 @@ struct Plan {
   int64_t piece;
   bool small;
   int lw = 0;
-  int64_t o_wslab = 0, o_count, o_sums, o_some, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_hct, o_part, o_zt, o_lse2, o_g, o_db64, o_dl, o_dlt, o_wt, o_slab, o_dbp;
+  int64_t o_wslab = 0, o_count, o_sums, o_some, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_hct, o_part, o_zt, o_lse2, o_g, o_db64, o_dbe, o_dl, o_dlt, o_wt, o_slab, o_dbp;
   int64_t take(int64_t n) {
     const int64_t at = bytes;
     bytes += up(n, 256);
@@ -1119,7 +1113,7 @@ struct Plan {
     while (kp < topk) kp *= 2;
     small = rows <= SMALL_ROWS || npad / 256 * ((vocab + 255) / 256) <= SMALL_TILES;
     const int bm = small ? Small::BM : Big::BM;
-    o_count = take(12);                                        // the largest weight, `arrived`
+    o_count = take(8);                                         // and `arrived`
     o_sums = take(npad / 16 * 8);
     o_some = topk ? take(npad * 4) : 0;
     o_rowmap = take(npad * 4);
@@ -1135,10 +1129,10 @@ struct Plan {
     o_lse2 = take(npad * 4);
     o_g = take(npad * 4);
     piece = piece_cols;
-    o_hct = o_db64 = o_dl = o_dlt = o_slab = o_dbp = 0;
+    o_hct = o_db64 = o_dbe = o_dl = o_dlt = o_slab = o_dbp = 0;
     o_wt = -1;
     if (piece) {
-      if (topk) o_db64 = take((int64_t)vocab * 8);
+      if (topk) o_db64 = take((int64_t)vocab * 8), o_dbe = take((int64_t)vocab * 4);
       o_hct = take((int64_t)hp * npad * 2);
       o_dl = take(npad * piece * 2);
       o_dlt = take(npad * piece * 2);
@@ -1285,7 +1279,7 @@ int linear_loss(const LinearLoss& c, hipStream_t st) {
   a.tgt_idx0 = (int*)(w + P.o_ti0); a.tgt_q0 = (float*)(w + P.o_tq0); a.tgt_idx = (int*)(w + P.o_ti); a.tgt_q = (float*)(w + P.o_tq);
   a.hc = (bf16_t*)(w + P.o_hc); a.hct = (bf16_t*)(w + P.o_hct); a.part = (float2*)(w + P.o_part); a.zt = (float*)(w + P.o_zt); a.tgt_z = (float*)(w + P.o_tz); a.lse2 = (float*)(w + P.o_lse2); a.g = (float*)(w + P.o_g);
   a.dl = (bf16_t*)(w + P.o_dl); a.dlt = (bf16_t*)(w + P.o_dlt); a.wt = P.o_wt >= 0 && c.d_hidden ? (bf16_t*)(w + P.o_wt) : nullptr; a.slab = (float*)(w + P.o_slab); a.wslab = (float*)(w + P.o_wslab); a.lw = P.lw; a.dbp = (float*)(w + P.o_dbp); a.vpad = P.vpad;
-  a.wmax = (float*)(a.count + 1); a.arrived = (unsigned*)(a.count + 2); a.sums = (double*)(w + P.o_sums); a.db64 = (unsigned long long*)(w + P.o_db64);
+  a.arrived = (unsigned*)(a.count + 1); a.sums = (double*)(w + P.o_sums); a.db64 = (unsigned long long*)(w + P.o_db64); a.dbe = (unsigned*)(w + P.o_dbe);
   a.piece = (int)piece;
   int num_cu = 0;
   CACO_TRY_RC(prepare_launch(reinterpret_cast<const void*>(&lse_kernel<Big>), Big::SMEM_WFAR, &num_cu));
