@@ -65,7 +65,7 @@ struct LossArgs {
   int reduction;
   const float* row_weight;
   const float* grad_scale;
-  float *row_loss, *lse, *loss;
+  float *row_loss, *lse, *lse_rest, *loss;      // lse_rest: what the rounding of lse to fp32 leaves, or null
   bf16_t* dh; int64_t ld_dh;
   bf16_t* dw; int64_t ld_dw;
   float* db;
@@ -79,9 +79,10 @@ struct LossArgs {
   bf16_t* hc;                        // [npad, hp]
   bf16_t* hct;                       // [hp, npad]: its transpose, for d weight
   float2* part;                      // (max, sum) of log2-logits, [group of row blocks][workgroup][rows of a block]
-  float* zt;                         // cross entropy: the label's logit; distillation: sum_k q_k (z_k / T - log q_k), log2 units
-  float* tgt_z;                      // distillation: the entries' log2-logits [npad, kp]
-  float *lse2, *g;                   // compact: lse in log2 units, the row's weight in the gradients
+  float* zt;                         // cross entropy: the label's logit
+  float* tgt_z;                      // distillation: the entries' logits [npad, kp]
+  // compact: lse in log2 units is lse2 + a rest of at most 0.6 (see split_lse); the row's weight in the gradients g, and g 2^-rest
+  float *lse2, *g, *gr;
   // distillation, d bias: per word the exponent field of the largest |g q| of its entries, and their sum as an integer (see targets2_kernel)
   unsigned* dbe; unsigned long long* db64;
   // d logits of the piece in blocks of 256 rows x 256 columns, [row block][column block][256][256], once with the columns next to one another
@@ -291,8 +292,14 @@ __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, i
   if (backward && blockIdx.y == 0 && t < 64) {
     const bool real = c0 + t < n;
     const int64_t row = real ? rowmap[c0 + t] : 0;
-    a.g[c0 + t] = real && common_scale(a, n) != 0.f ? a.row_weight ? a.row_weight[row] : 1.f : 0.f;
-    if (from_lse) a.lse2[c0 + t] = real ? a.lse[row] * LOG2E : 0.f;
+    const float g = real && common_scale(a, n) != 0.f ? a.row_weight ? a.row_weight[row] : 1.f : 0.f;
+    a.g[c0 + t] = g;
+    if (from_lse) {
+      const double l = real ? ((double)a.lse[row] + (a.lse_rest ? (double)a.lse_rest[row] : 0.)) * 1.4426950408889634074 : 0.;
+      const float l2 = (float)l;
+      a.lse2[c0 + t] = l2;
+      a.gr[c0 + t] = g * __builtin_amdgcn_exp2f(-(float)(l - (double)l2));
+    }
   }
 }
 
@@ -319,59 +326,52 @@ __global__ __launch_bounds__(256) void transpose_kernel(const bf16_t* src, int64
   }
 }
 
-// (distillation) sum_k q_k (log q_k - z_k / T) of a compact row: 16 lanes per entry, the entries' rows of weight gathered.
-// In log2 units, as `finish` has them.  A row with 16 entries or more has four waves: what it takes is the gathers' latency, and one wave
-// after the other through 100 entries took 61 us for 1000 rows, four waves 25.
+// (distillation) The entries' logits: a wave takes 16 entries of a compact row at a time, their rows of weight gathered.  The same instruction
+// as in the tiles, over k in the same order and from the same first sum, so that an entry has the bits its word's logit has in `lse` and `dlogits`:
+// what is left when it is taken from the row's reference has no rounding at the logits' size.  15 of the 16 columns of a product are
+// spent for that; what the kernel takes is the gathers' latency (16 rows x 64 bytes in one load, eight loads on their way).
 // With d bias, each entry also leaves its exponent with its word.
-constexpr int target_waves(int kp) { return kp >= 16 ? 4 : 1; }
+constexpr int target_waves(int kp) { return kp > 32 ? 4 : kp > 16 ? 2 : 1; }      // waves of a row
 __global__ __launch_bounds__(256) void target_logits_kernel(LossArgs a) {
-  __shared__ float s_sum[4];
-  const int lane = threadIdx.x & 63, l16 = lane & 15, grp = lane >> 4, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4, wave = threadIdx.x >> 6;
   const int waves = target_waves(a.kp), part = wave & (waves - 1);
-  const int64_t c = waves == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
-  const bool real = c < *a.count;
-  float sum = 0.f;
-  if (real) {
-    const bf16_t* h = a.hc + c * a.hp;
-    const float g = a.db ? a.g[c] : 0.f;
-    const int share = a.kp / waves;                       // up to 32 entries of this wave, in steps of four
-    const int at = l16 * 4 + grp;                         // lane (step, group) brings that step's entry of the group: all of them at once
-    const int64_t first = c * a.kp + part * share;
-    const int idx0 = at < share ? a.tgt_idx[first + at] : -1;
-    const float q0 = at < share ? a.tgt_q[first + at] : 0.f;
-    const int steps = (share + 3) / 4;
-    for (int s = 0; s < steps; ++s) {
-      const int idx = __shfl(idx0, grp * 16 + s, 64);
-      const float q = __shfl(q0, grp * 16 + s, 64);
-      float z = 0.f;
-      if (idx >= 0) {
-        const bf16_t* w = a.weight + (int64_t)idx * a.ld_w;
-        for (int i = l16 * 8; i < a.dim; i += 128) {
-          const bf16x8 x = *reinterpret_cast<const bf16x8*>(h + i), y = *reinterpret_cast<const bf16x8*>(w + i);
+  const int64_t c = (int64_t)blockIdx.x * (4 / waves) + wave / waves;
+  if (c >= *a.count) return;
+  const bf16_t* h = a.hc + c * a.hp;
+  const float g = a.db ? a.g[c] : 0.f;
+  for (int e0 = part * 16; e0 < a.kp; e0 += 16 * waves) {
+    const int64_t first = c * a.kp + e0;
+    const int idx = e0 + l16 < a.kp ? a.tgt_idx[first + l16] : -1;      // of the row of weight that this lane brings
+    const bf16_t* w = a.weight + (int64_t)max(idx, 0) * a.ld_w;
+    const float b = a.bias && idx >= 0 ? a.bias[idx] : 0.f;
+    f32x4 acc;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) z = __builtin_fmaf((float)x[e], (float)y[e], z);
-        }
+    for (int e = 0; e < 4; ++e) acc[e] = __shfl(b, lq * 4 + e, 64);
+    for (int k0 = 0; k0 < a.dim; k0 += 256) {
+      bf16x8 x[8], y[8];      // an absent entry reads word 0, its logit is not used
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int k = k0 + u * 32 + lq * 8;
+        x[u] = *reinterpret_cast<const bf16x8*>(h + min(k, a.dim - 8));
+        y[u] = *reinterpret_cast<const bf16x8*>(w + min(k, a.dim - 8));
       }
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
-      if (q != 0.f && l16 == 0) {      // 0 log 0 = 0: an entry of weight 0 (or none) adds nothing, whatever its logit is
-        if (a.bias) z += a.bias[idx];
-        z *= a.inv_t * LOG2E;
-        sum += q * (log2f(q) - z);
-        a.tgt_z[first + s * 4 + grp] = z;
-        if (g != 0.f) {
-          const unsigned x = max(float_exponent(g * q), 1u);      // below the normal numbers the units stay the same
-          if (a.dbe[idx] < x) atomicMax(a.dbe + idx, x);          // it only grows: an old value costs an atomic, not an answer
-        }
+      for (int u = 0; u < 8; ++u) {
+        if (k0 + u * 32 + lq * 8 >= a.dim) x[u] = y[u] = bf16x8{};
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[u], x[u], acc, 0, 0, 0);
       }
     }
-    sum = wave_sum(sum);
-  }
-  if (lane == 0) s_sum[wave] = sum;
-  __syncthreads();
-  if (real && lane == 0 && part == 0) {
-    if (waves == 4) sum = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-    a.zt[c] = -sum;
+    // every column holds the row's logits, those of entries lq * 4 .. + 3 in this lane: lanes l16 = 0 .. 3 take one each
+    const int entry = lq * 4 + l16;
+    if (l16 >= 4 || e0 + entry >= a.kp) continue;
+    const float z = l16 == 0 ? acc[0] : l16 == 1 ? acc[1] : l16 == 2 ? acc[2] : acc[3];
+    a.tgt_z[first + entry] = z;
+    const int word = a.tgt_idx[first + entry];
+    const float q = a.tgt_q[first + entry];
+    if (word >= 0 && g != 0.f && q != 0.f) {
+      const unsigned x = max(float_exponent(g * q), 1u);      // below the normal numbers the units stay the same
+      if (a.dbe[word] < x) atomicMax(a.dbe + word, x);        // it only grows: an old value costs an atomic, not an answer
+    }
   }
 }
 
@@ -434,14 +434,14 @@ struct Walk {
 // groups of at most `rb` row blocks
 __host__ __device__ inline int64_t most_groups(int64_t rb) { return rb / 8 + 3; }
 
-// The words of an output tile: bias of its columns, labels (and for d logits lse and g) of its rows.
+// The words of an output tile: bias of its columns, labels (and for d logits lse, g and g 2^-rest) of its rows.
 template <typename C>
 struct Words {
-  static constexpr int BIAS = 0, Y = C::BN * 4, LSE = Y + C::BM * 4, G = LSE + C::BM * 4;
+  static constexpr int BIAS = 0, Y = C::BN * 4, LSE = Y + C::BM * 4, G = LSE + C::BM * 4, GR = G + C::BM * 4;
   static __device__ __forceinline__ void bring(const LossArgs& a, int n0, int64_t m0, bool grad, char* lds) {
     const int lane = vg_lane();
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int pc = wave; pc < (C::BN + (grad ? 3 : 1) * C::BM) / 64; pc += C::WAVES) {
+    for (int pc = wave; pc < (C::BN + (grad ? 4 : 1) * C::BM) / 64; pc += C::WAVES) {
       if (pc < C::BN / 64) {
         if (a.bias) vg_words(a.bias + min(n0 + pc * 64, a.vocab), a.vocab - n0 - pc * 64, lds + BIAS + pc * 256, lane);
         continue;
@@ -450,6 +450,7 @@ struct Words {
       if (which == 0 && !a.topk) vg_words(a.tgt_idx + m0 + m, 64, lds + Y + m * 4, lane);
       if (which == 1) vg_words(a.lse2 + m0 + m, 64, lds + LSE + m * 4, lane);
       if (which == 2) vg_words(a.g + m0 + m, 64, lds + G + m * 4, lane);
+      if (which == 3) vg_words(a.gr + m0 + m, 64, lds + GR + m * 4, lane);
     }
   }
   // sums begin with the bias; a column past the vocabulary with -inf, its logit and nothing else comes of it
@@ -472,8 +473,9 @@ struct Words {
 };
 
 // Per element one multiply-add, one v_exp_f32 and one addition.  The reference of a lane's row is the maximum over the row's first tile of
-// this wave (four lanes share it) and stays there while the sums stay below 2^100; when one does not (or is NaN) the whole wave goes
-// over the tile again with its maxima.  Logits far below the reference add what they should: nothing.
+// this wave (four lanes share it) and stays there while a tile adds less than 2^8; when one does not (or is NaN) the whole wave goes
+// over the tile again with its maxima.  Logits far below the reference add what they should: nothing.  No exponent passes 8, so its
+// rounding stays below 2^-22 whatever the logits' size; and a reference that moves has grown by 4 at least, which few tiles see.
 template <typename C>
 __device__ __forceinline__ void lse_body(const LossArgs& a, char* smem) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -510,13 +512,13 @@ __device__ __forceinline__ void lse_body(const LossArgs& a, char* smem) {
         const int n0 = tn * C::BN + wn * 16 * C::NI + lq * 4;      // this lane's columns: n0 + j * 16 + e
 #pragma unroll
         for (int q = 0; q < C::MI; ++q) {
-          float s[4] = {sm[q], 0.f, 0.f, 0.f};
+          float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int j = 0; j < C::NI; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[q][j][e], cs, nref[q]));
           s[0] = (s[0] + s[1]) + (s[2] + s[3]);
-          if (__ballot(!(s[0] < 0x1p100f))) {
+          if (__ballot(!(s[0] < 0x1p8f))) {
             float m = -nref[q];
 #pragma unroll
             for (int j = 0; j < C::NI; ++j)
@@ -524,14 +526,15 @@ __device__ __forceinline__ void lse_body(const LossArgs& a, char* smem) {
               for (int e = 0; e < 4; ++e) m = fmaxf(m, acc[q][j][e] * cs);
             m = fmaxf(m, __shfl_xor(m, 16, 64));
             m = fmaxf(m, __shfl_xor(m, 32, 64));
-            s[0] = sm[q] * __builtin_amdgcn_exp2f(-nref[q] - m);
+            sm[q] *= __builtin_amdgcn_exp2f(-nref[q] - m);
+            s[0] = 0.f;
 #pragma unroll
             for (int j = 0; j < C::NI; ++j)
 #pragma unroll
               for (int e = 0; e < 4; ++e) s[0] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[q][j][e], cs, -m));
             nref[q] = -m;
           }
-          sm[q] = s[0];
+          sm[q] += s[0];
         }
         if (label) {
 #pragma unroll
@@ -589,6 +592,19 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
   lse_body<C>(a, smem);
 }
 
+// log2 of the sum s 2^m as `whole` + `rest`.  With s = f 2^k, 0.75 <= f < 1.5, it is m + k + log2 f: `whole` is m + k rounded, `rest` log2 f and
+// what that rounding lost, so the two together are good to a rounding of f.  One number would be good to a rounding of m, and all that
+// is left of a confident row, log2 s of its loss and 1 - p of its gradient, would go under where the logits have a large part in common.
+__device__ __forceinline__ void split_lse(float m, float s, float& k, float& lf, float& whole, float& rest) {
+  const unsigned u = __float_as_uint(s);
+  const int e = u - 0x00800000u < 0x7f000000u ? (int)((u + 0x00400000u) >> 23) - 127 : 0;      // positive, normal, finite; others stay as they are
+  k = (float)e;
+  lf = log1pf(ldexpf(s, -e) - 1.f) * LOG2E;
+  whole = m + k;
+  const float b = whole - m;
+  rest = (m - (whole - b)) + (k - b) + lf;
+}
+
 // One wave: joins the parts of one of the caller's rows, row loss (returned, too) and lse; rows that do not count get zeros.
 template <typename C>
 __device__ __forceinline__ float finish_row(const LossArgs& a, int wgs, int64_t row) {
@@ -598,6 +614,7 @@ __device__ __forceinline__ float finish_row(const LossArgs& a, int wgs, int64_t 
     if (lane == 0) {
       a.row_loss[row] = 0.f;
       if (a.lse) a.lse[row] = 0.f;
+      if (a.lse_rest) a.lse_rest[row] = 0.f;
     }
     return 0.f;
   }
@@ -644,12 +661,33 @@ __device__ __forceinline__ float finish_row(const LossArgs& a, int wgs, int64_t 
     s = s * __builtin_amdgcn_exp2f(m - nm) + os * __builtin_amdgcn_exp2f(om - nm);
     m = nm;
   }
-  // the target is taken from the reference first: what a confident row loses is not rounded at the logits' size
-  const float ls = log2f(s), l2 = m + ls, d = a.topk ? m - a.zt[c] : __builtin_fmaf(-a.zt[c], a.inv_t * LOG2E, m);
-  const float loss = (d + ls) * LN2 * a.temperature * a.temperature;
+  float k, lf, whole, rest;
+  split_lse(m, s, k, lf, whole, rest);
+  // -log2 of a word's probability: its logit is taken from the reference first, so nothing is rounded at the logits' size
+  const float cs = a.inv_t * LOG2E;
+  const auto minus_log2_p = [&](float z) { return (__builtin_fmaf(-z, cs, m) + k) + lf; };
+  float d;
+  if (!a.topk) {
+    d = minus_log2_p(a.zt[c]);
+  } else {
+    d = 0.f;
+    for (int i = lane; i < a.kp; i += 64) {
+      const float q = a.tgt_q[(int64_t)c * a.kp + i];
+      if (q != 0.f) d += q * (log2f(q) + minus_log2_p(a.tgt_z[(int64_t)c * a.kp + i]));      // 0 log 0 = 0, whatever the logit is
+    }
+    d = wave_sum(d);
+  }
+  const float loss = d * LN2 * a.temperature * a.temperature;
   if (lane == 0) {
-    a.lse2[c] = l2;
-    if (a.lse) a.lse[row] = l2 * LN2;
+    if (a.gr) {
+      a.lse2[c] = whole;
+      a.gr[c] = a.g[c] * __builtin_amdgcn_exp2f(-rest);
+    }
+    if (a.lse) {
+      const double l = ((double)whole + (double)rest) * 0.69314718055994530942;
+      a.lse[row] = (float)l;
+      if (a.lse_rest) a.lse_rest[row] = fabsf((float)l) < INFINITY ? (float)(l - (double)(float)l) : 0.f;
+    }
     a.row_loss[row] = loss;
   }
   return loss;
@@ -753,6 +791,7 @@ __device__ __forceinline__ void dlogits_body(const LossArgs& a, char* smem) {
             for (int u = 0; u < 2; ++u) {
               const int q = q2 * 2 + u, row = (wm * C::MI + q) * 16 + l16;
               const float nl = -*reinterpret_cast<const float*>(w + Words<C>::LSE + row * 4), g = *reinterpret_cast<const float*>(w + Words<C>::G + row * 4);
+              const float gr = *reinterpret_cast<const float*>(w + Words<C>::GR + row * 4);
               f32x4 p[Turn::NJ];
 #pragma unroll
               for (int j = 0; j < Turn::NJ; ++j) p[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -760,7 +799,7 @@ __device__ __forceinline__ void dlogits_body(const LossArgs& a, char* smem) {
 #pragma unroll
                 for (int j = 0; j < Turn::NJ; ++j)
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) p[j][e] = g * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[q][h * Turn::NJ + j][e], cs, nl));
+                  for (int e = 0; e < 4; ++e) p[j][e] = gr * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[q][h * Turn::NJ + j][e], cs, nl));
                 if (label) {
                   const int d = *reinterpret_cast<const int*>(w + Words<C>::Y + row * 4) - n0 - h * Turn::NJ * 16;
                   if ((unsigned)d < 16u * Turn::NJ && (d & 12) == 0) {
@@ -817,7 +856,7 @@ __global__ __launch_bounds__(256) void targets2_kernel(LossArgs a) {
   const int idx = a.tgt_idx[t], v = idx - a.v0;
   const float g = a.g[c], q = a.tgt_q[t];
   if (idx < 0 || v < 0 || v >= a.piece || g == 0.f || q == 0.f) return;
-  const bf16_t d = (bf16_t)(g * __builtin_amdgcn_exp2f(a.tgt_z[t] - a.lse2[c]) - g * q);
+  const bf16_t d = (bf16_t)(a.gr[c] * __builtin_amdgcn_exp2f(__builtin_fmaf(a.tgt_z[t], a.inv_t * LOG2E, -a.lse2[c])) - g * q);
   const int64_t block = dl_block(a, c, v);
   a.dl[block + (c & 255) * 256 + (v & 255)] = d;
   if (a.dw) a.dlt[block + (v & 255) * 256 + (c & 255)] = d;
@@ -1099,7 +1138,7 @@ struct Plan {
   int64_t piece;
   bool small;
   int lw = 0;
-  int64_t o_wslab = 0, o_count, o_sums, o_some, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_hct, o_part, o_zt, o_lse2, o_g, o_db64, o_dbe, o_dl, o_dlt, o_wt, o_slab, o_dbp;
+  int64_t o_wslab = 0, o_count, o_sums, o_some, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_hct, o_part, o_zt, o_lse2, o_g, o_gr, o_db64, o_dbe, o_dl, o_dlt, o_wt, o_slab, o_dbp;
   int64_t take(int64_t n) {
     const int64_t at = bytes;
     bytes += up(n, 256);
@@ -1126,12 +1165,13 @@ struct Plan {
     o_hc = take(npad * hp * 2);
     o_part = take(most_groups(npad / bm) * (small ? MAX_WG : MAX_CU) * bm * 8);
     o_zt = take(npad * 4);
-    o_lse2 = take(npad * 4);
-    o_g = take(npad * 4);
     piece = piece_cols;
-    o_hct = o_db64 = o_dbe = o_dl = o_dlt = o_slab = o_dbp = 0;
+    o_lse2 = o_g = o_gr = o_hct = o_db64 = o_dbe = o_dl = o_dlt = o_slab = o_dbp = 0;
     o_wt = -1;
     if (piece) {
+      o_lse2 = take(npad * 4);
+      o_g = take(npad * 4);
+      o_gr = take(npad * 4);
       if (topk) o_db64 = take((int64_t)vocab * 8), o_dbe = take((int64_t)vocab * 4);
       o_hct = take((int64_t)hp * npad * 2);
       o_dl = take(npad * piece * 2);
@@ -1180,14 +1220,13 @@ int launch(const char* what, K kern, dim3 grid, int threads, int lds, hipStream_
 template <typename C>
 int run_loss(LossArgs& a, const Plan& P, int what, int cus, hipStream_t st) {
   const dim3 rows4((unsigned)((a.rows + 3) / 4));
-  const dim3 pad4((unsigned)(P.npad / 4));
   const int wgs = P.small ? 2 * cus : cus;
   const bool fwd = what & CACO_LOSS_FORWARD, bwd = what & CACO_LOSS_BACKWARD;
   if (a.topk && a.rows) CACO_TRY_RC(launch("loss targets", targets_kernel, rows4, 256, 0, st, a));
   const bool few = a.rows <= FEW_ROWS;
   if (!few) CACO_TRY_RC(launch("loss compact", compact_kernel, dim3(1), 1024, 0, st, a));
   CACO_TRY_RC(launch("loss gather", few ? gather_kernel<true> : gather_kernel<false>, dim3((unsigned)(P.npad / 64), a.hp / 64), 256, 0, st, a, (int)bwd, (int)!fwd));
-  if (a.topk) CACO_TRY_RC(launch("loss target logits", target_logits_kernel, target_waves(a.kp) == 4 ? dim3((unsigned)P.npad) : pad4, 256, 0, st, a));
+  if (a.topk) CACO_TRY_RC(launch("loss target logits", target_logits_kernel, dim3((unsigned)(P.npad / (4 / target_waves(a.kp)))), 256, 0, st, a));
   if (fwd) {
     CACO_TRY_RC(launch("loss lse", lse_kernel<C>, dim3(wgs), C::THREADS, C::SMEM_WFAR, st, a));
     const int64_t fin = (a.rows + 15) / 16;
@@ -1230,7 +1269,7 @@ int64_t linear_loss_workspace(int64_t rows, int32_t vocab, int32_t dim, int32_t 
 
 int linear_loss(const LinearLoss& c, hipStream_t st) {
   CACO_TRY_RC(check_sizes(c.rows, c.vocab, c.dim, c.topk));
-  CACO_REQUIRE(c.what >= 1 && c.what <= 3, "linear loss: `what` must be CACO_LOSS_FORWARD, CACO_LOSS_BACKWARD or both");
+  CACO_REQUIRE((c.what & 3) && !(c.what & ~7), "linear loss: `what` must be CACO_LOSS_FORWARD, CACO_LOSS_BACKWARD or both, with CACO_LOSS_LSE_PAIR or without");
   CACO_REQUIRE(c.reduction >= CACO_REDUCE_NONE && c.reduction <= CACO_REDUCE_SUM, "linear loss: unknown reduction %d", c.reduction);
   CACO_REQUIRE(c.weight && c.ws && (c.rows == 0 || (c.hidden && (c.topk ? c.teacher && c.teacher_idx : c.labels != nullptr))), "linear loss: null argument");
   CACO_REQUIRE(c.topk == 0 || (c.temperature > 0.f && c.temperature < INFINITY), "linear loss: temperature must be positive and finite");
@@ -1272,12 +1311,13 @@ int linear_loss(const LinearLoss& c, hipStream_t st) {
   a.inv_t = 1.f / a.temperature;
   a.rows = c.rows; a.npad = P.npad; a.vocab = c.vocab; a.dim = c.dim; a.hp = P.hp;
   a.reduction = c.reduction; a.row_weight = c.row_weight; a.grad_scale = c.grad_scale;
-  a.row_loss = c.row_loss; a.lse = c.lse; a.loss = c.loss;
+  a.row_loss = c.row_loss; a.lse = c.lse; a.lse_rest = c.lse && (c.what & CACO_LOSS_LSE_PAIR) ? c.lse + c.rows : nullptr; a.loss = c.loss;
   a.dh = bwd ? c.d_hidden : nullptr; a.ld_dh = c.ld_dh; a.dw = bwd ? c.d_weight : nullptr; a.ld_dw = c.ld_dw; a.db = bwd ? c.d_bias : nullptr;
   char* w = reinterpret_cast<char*>(c.ws);
   a.count = (int*)(w + P.o_count); a.some = (int*)(w + P.o_some); a.rowmap = (int*)(w + P.o_rowmap); a.inv = (int*)(w + P.o_inv);
   a.tgt_idx0 = (int*)(w + P.o_ti0); a.tgt_q0 = (float*)(w + P.o_tq0); a.tgt_idx = (int*)(w + P.o_ti); a.tgt_q = (float*)(w + P.o_tq);
-  a.hc = (bf16_t*)(w + P.o_hc); a.hct = (bf16_t*)(w + P.o_hct); a.part = (float2*)(w + P.o_part); a.zt = (float*)(w + P.o_zt); a.tgt_z = (float*)(w + P.o_tz); a.lse2 = (float*)(w + P.o_lse2); a.g = (float*)(w + P.o_g);
+  a.hc = (bf16_t*)(w + P.o_hc); a.hct = (bf16_t*)(w + P.o_hct); a.part = (float2*)(w + P.o_part); a.zt = (float*)(w + P.o_zt); a.tgt_z = (float*)(w + P.o_tz); 
+  a.lse2 = (float*)(w + P.o_lse2); a.g = (float*)(w + P.o_g); a.gr = bwd ? (float*)(w + P.o_gr) : nullptr;
   a.dl = (bf16_t*)(w + P.o_dl); a.dlt = (bf16_t*)(w + P.o_dlt); a.wt = P.o_wt >= 0 && c.d_hidden ? (bf16_t*)(w + P.o_wt) : nullptr; a.slab = (float*)(w + P.o_slab); a.wslab = (float*)(w + P.o_wslab); a.lw = P.lw; a.dbp = (float*)(w + P.o_dbp); a.vpad = P.vpad;
   a.arrived = (unsigned*)(a.count + 1); a.sums = (double*)(w + P.o_sums); a.db64 = (unsigned long long*)(w + P.o_db64); a.dbe = (unsigned*)(w + P.o_dbe);
   a.piece = (int)piece;

@@ -29,7 +29,7 @@ from .model import _ptr, _stream
 
 Tensor = torch.Tensor
 
-FORWARD, BACKWARD = 1, 2
+FORWARD, BACKWARD, LSE_PAIR = 1, 2, 4
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 # d logits of one piece of the vocabulary, bf16, by rows and by columns: 8192 tokens x 50265 words are one piece, 0.6 % of a card's memory
 PIECE_BYTES = 2 << 30
@@ -136,9 +136,9 @@ def _call(head: _Head, target: dict, what: int, *, ignore_index: int = -100, red
 def _forward(head: _Head, target: dict, ignore_index: int, keep_lse: bool):
     new = lambda *s: torch.empty(*s, dtype=torch.float32, device=head.device)
     row_loss = new(head.rows)
-    lse = new(head.rows) if keep_lse else None
+    lse = new(2, head.rows) if keep_lse else None      # with the rest that its rounding leaves: a confident row's gradient needs it
     loss = new(()) if head.reduction else None
-    _call(head, target, FORWARD, ignore_index=ignore_index, row_loss=row_loss, lse=lse, loss=loss)
+    _call(head, target, FORWARD | LSE_PAIR, ignore_index=ignore_index, row_loss=row_loss, lse=lse, loss=loss)
     return (row_loss.reshape(head.lead) if loss is None else loss), lse
 
 
@@ -163,7 +163,7 @@ class _LinearLoss(torch.autograd.Function):
             dh, dw, db = new(0, hidden), new(1, weight), new(2, bias)
             grad = grad.to(torch.float32).contiguous()
             kw = {"grad_scale": grad} if head.reduction else {"row_weight": grad.reshape(-1)}
-            _call(head, ctx.target, BACKWARD, ignore_index=ctx.ignore_index, lse=ctx.lse, d_hidden=dh, d_weight=dw, d_bias=db,
+            _call(head, ctx.target, BACKWARD | LSE_PAIR, ignore_index=ctx.ignore_index, lse=ctx.lse, d_hidden=dh, d_weight=dw, d_bias=db,
                   piece_bytes=ctx.piece_bytes, **kw)
         return dh, dw, db, None, None, None, None
 

@@ -216,6 +216,9 @@ void caco_decode_end(caco_decode_state* s);
  *   writes the gradients of that scalar times *grad_scale_dev (for CACO_REDUCE_NONE: of the weighted sum): d_hidden_dev bf16
  *   [rows, dim] (ld_dh), d_weight_dev bf16 [vocab, dim] (ld_dw), d_bias_dev fp32 [vocab]; each may be NULL, not all.  It reads lse_dev
  *   unless the forward pass is part of the same call (CACO_LOSS_FORWARD | CACO_LOSS_BACKWARD).  No row counts: zero gradients.
+ *   With CACO_LOSS_LSE_PAIR in both calls lse_dev is fp32 [2, rows]: the rows' lse, then what its rounding to fp32 lost.  Without it the
+ *   backward pass of a later call has every probability to |lse| 2^-24 only, which is all that 1 - p of a confident row may be; a call that does both
+ *   passes has the pair by itself.
  *   row_weight_dev fp32 [rows] or NULL (= 1), grad_scale_dev fp32 [1] or NULL (= 1).
  * Row strides are in elements, >= dim and multiples of 8, and rows start at multiples of 16 bytes; dim is a multiple of 8; rows <= 2^22
  *   (0 is allowed), vocab <= 2^24, rows * vocab <= 2^46 (both rounded up to 256), dim <= 65536.
@@ -225,6 +228,7 @@ void caco_decode_end(caco_decode_state* s);
  * Capturable into a graph: no synchronisation, no allocation, no memset; equal calls give equal bits. */
 #define CACO_LOSS_FORWARD 1
 #define CACO_LOSS_BACKWARD 2
+#define CACO_LOSS_LSE_PAIR 4
 #define CACO_REDUCE_NONE 0
 #define CACO_REDUCE_MEAN 1
 #define CACO_REDUCE_SUM 2

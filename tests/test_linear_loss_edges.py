@@ -73,3 +73,148 @@ def test_d_bias_with_weights_that_lie_far_apart(call):
     # the same word in the heaviest and in the lightest row: the sum is as exact as fp32 sums are
     x["idx"][:, 0] = 100
     close(call(x, reduction="sum", row_weight=wt), expect(x, reduction="sum", row_weight=wt), "one word of all rows")
+
+
+# ------------------------------------------------------------------------------------------------------------------------------------
+# confident rows: what is left of 1 - p does not depend on what all logits have in common
+# ------------------------------------------------------------------------------------------------------------------------------------
+def confident(offset, topk=0, rows=48, vocab=300, dim=64):
+    """Rows whose label's logit is about 14 above the others', so that 1 - p is near 1e-5; bias = offset for every word.  Distillation: a teacher
+    that is certain of the same word."""
+    x = make(rows, vocab, dim, topk=topk, seed=73, ignored=0.0, spread=0.5)
+    y = torch.arange(rows) * 3
+    w = x["w"].float()
+    scale = 20.0 / (w[y] ** 2).sum(1, keepdim=True)
+    x["h"] = (0.3 * x["h"].float() + scale * w[y]).bfloat16()
+    x["b"] = torch.full((vocab,), float(offset))
+    if topk:
+        x["idx"] = (y[:, None] + torch.arange(topk)) % vocab
+        x["teacher"] = torch.where(torch.arange(topk) == 0, 12.0, -2.0) - torch.linspace(0, 1, topk)[None, :].repeat(rows, 1)
+    else:
+        x["y"] = y
+    return x
+
+
+def expect_confident(x, row_weight=None):
+    """The gradients of the summed loss and what they may be off by when a row's statistics and its probabilities come from the same logits.
+
+    Errors dz of the logits (at most (D + 1) u32 S, S = |h| . |w| + |b|) move p_v by p_v |dz_v - sum_u p_u dz_u|, that is by p_v (1 - p_v) 2 max dz, and
+    the loss, sum_k q_k (lse - z_k), by sum_v |p_v - q_v| max dz.  What the logits have in common is only in that.  Exponents are within 2^-22 of
+    the difference that they round where it is below 8 (which is where p matters) and within u32 of it elsewhere; the sum of the exponentials is 300 terms in
+    at most 24 additions one after the other; exp2, log2 and products are good to 8 u32:  p off by 40 u32 (1 + |log p| / 16) p, the loss by
+    40 u32 (1 + sum_k q_k (|log q_k| + |log p_k|)).  q: as in `expect`, 64 u32 (|t| + 8).  Then one rounding to bf16 each, and for the distillation's d bias
+    sums of p and of q apart: 64 u32 (p + q)."""
+    h, w, b = x["h"].double(), x["w"].double(), x["b"].double()
+    R, V, D = h.shape[0], w.shape[0], h.shape[1]
+    q, _ = targets(x, 1.0)
+    z = h @ w.T + b
+    dmax = ((D + 1) * U32 * (h.abs() @ w.abs().T + b.abs())).amax(1, keepdim=True)
+    lp = torch.log_softmax(z, 1)
+    p = lp.exp()
+    own = 64 * U32 * (x["teacher"].double().abs().amax(1, keepdim=True) + 8) if x["topk"] else torch.zeros(R, 1, dtype=torch.float64)
+    loss = (torch.special.xlogy(q, q) - q * lp).sum(1)
+    out = {"row_loss": (loss, ((p - q).abs().sum(1, keepdim=True) * dmax).squeeze(1)
+                        + (own * q * (1 - q) * (1 + torch.where(q > 0, torch.log(q.clamp_min(1e-300)) - lp, 0.0).abs())).sum(1)
+                        + 40 * U32 * (1 + (torch.special.xlogy(q, q).abs() - q * lp).sum(1)))}
+    dL = p - q
+    # a word that is certain is off by own * (1 - q), as a probability is
+    raw = p * (1 - p) * 2 * dmax * 1.01 + 40 * U32 * (1 + lp.abs() / 16) * p + own * q * (1 - q) + 4 * U32 * q
+    dLt = raw + 2.0 ** -8 * (dL.abs() + raw)
+    for name, val, tol in (("d_hidden", dL @ w, dLt @ w.abs() + (V + 64) * U32 * (dL.abs() @ w.abs())),
+                           ("d_weight", dL.T @ h, dLt.T @ h.abs() + (R + 64) * U32 * (dL.abs().T @ h.abs()))):
+        out[name] = (val, tol * (1 + 2.0 ** -8) + 2.0 ** -8 * val.abs() + 1e-38)
+    both = 64 * U32 * (p + q).sum(0) if x["topk"] else 0.0
+    out["d_bias"] = (dL.sum(0), raw.sum(0) + (R + 64) * U32 * dL.abs().sum(0) + both + 1e-38)
+    return out
+
+
+OFFSETS = [0.0, 60.0, 200.0, 3000.0, -3000.0]
+
+
+@pytest.mark.parametrize("call", WHERE, indirect=True)
+@pytest.mark.parametrize("offset", OFFSETS)
+@pytest.mark.parametrize("topk", [0, 5])
+def test_confident_rows_with_a_common_offset(call, topk, offset):
+    x = confident(offset, topk)
+    close(call(x, reduction="sum"), expect_confident(x), f"offset {offset}")
+
+
+def apart_on_simulator(x, T=1.0, reduction="mean", row_weight=None, pair=4):
+    """Forward and backward pass as two calls with a workspace each; the backward pass has lse only."""
+    from tests import simlib
+    lib, P = simlib.load(), simlib.ptr
+    R, D, V, K = x["h"].shape[0], x["h"].shape[1], x["w"].shape[0], x["topk"]
+    f = lambda *s: torch.full(s, float("nan"))
+    o = dict(row_loss=f(R), lse=f(2, R) if pair else f(R), loss=f(1), d_hidden=f(R, D).bfloat16(), d_weight=f(V, D).bfloat16(), d_bias=f(V))
+    red = {"none": 0, "mean": 1, "sum": 2}[reduction]
+    for what in (1, 2):
+        need = lib.caco_linear_loss_workspace(R, V, D, K, 1 << 30, what | pair)
+        ws = torch.full((need,), 0xFF, dtype=torch.uint8)
+        first = (what | pair, P(x["h"]), D, P(x["w"]), D, P(x["b"]))
+        fwd = what == 1
+        last = (R, V, D, red, P(row_weight), None, P(o["row_loss"]) if fwd else None, P(o["lse"]), P(o["loss"]) if fwd and red else None, P(o["d_hidden"]), D,
+                P(o["d_weight"]), D, P(o["d_bias"]), P(ws), need, None)
+        if K:
+            rc = lib.caco_linear_distill(*first, P(x["teacher"]), K, P(x["idx"]), K, x["idx"].element_size(), K, T, *last)
+        else:
+            rc = lib.caco_linear_ce(*first, P(x["y"]), -100, *last)
+        simlib.check(rc, "linear loss")
+    if pair:
+        o["lse"] = o["lse"].double().sum(0)
+    if not red:
+        del o["loss"]
+    return o
+
+
+def autograd_on_gpu(x, T=1.0, reduction="mean", row_weight=None):
+    d = dev(x)
+    for k in ("h", "w", "b"):
+        d[k].requires_grad_(True)
+    loss_of(d, T, reduction=reduction).backward()
+    return {"d_hidden": d["h"].grad, "d_weight": d["w"].grad, "d_bias": d["b"].grad}
+
+
+@pytest.mark.parametrize("offset", [200.0, 3000.0])
+@pytest.mark.parametrize("topk", [0, 5])
+@pytest.mark.parametrize("call", [pytest.param(apart_on_simulator, id="simulator"), pytest.param(autograd_on_gpu, id="gpu", marks=pytest.mark.gpu)])
+def test_confident_rows_with_a_backward_pass_of_its_own(request, call, topk, offset):
+    if call is apart_on_simulator:
+        request.getfixturevalue("sim")
+    x = confident(offset, topk)
+    close(call(x, reduction="sum"), expect_confident(x), f"offset {offset}")
+
+
+@pytest.mark.parametrize("topk", [0, 7])
+def test_simulator_two_calls(sim, topk):
+    """With the pair and with the single number; rows that do not count, all of them too."""
+    x = make(90, 700, 72, topk=topk, seed=74)
+    for pair in (4, 0):
+        close(apart_on_simulator(x, 2.0 if topk else 1.0, pair=pair), expect(x, 2.0 if topk else 1.0), f"pair {pair}")
+    o = apart_on_simulator(make(5, 300, 64, topk=topk, ignored=1.0, seed=5))
+    assert not o["lse"].any() and not o["d_weight"].any() and not o["d_bias"].any() and not o["d_hidden"].any()
+
+
+@pytest.mark.parametrize("call", WHERE, indirect=True)
+@pytest.mark.parametrize("rows,vocab,dim", [(70, 300, 72), (20, 2100, 328), (300, 700, 264)])
+def test_one_entry_is_the_cross_entropy(call, rows, vocab, dim):
+    """A teacher with one entry at T = 1 is a label: the entry's logit has the bits that the label's has in the tiles (whatever the large part that all
+    logits share), so the losses are equal bit for bit."""
+    x = make(rows, vocab, dim, seed=75)
+    x["b"] += 500.0
+    y = dict(x, topk=1, idx=x["y"][:, None].clone(), teacher=torch.randn(rows, 1))
+    a, b = call(x), call(y)
+    assert torch.equal(a["row_loss"], b["row_loss"]) and a["row_loss"].cpu().count_nonzero() == (x["y"] >= 0).sum()
+    close({k: v for k, v in b.items() if k != "lse"}, expect(y), "gradients")
+
+
+@pytest.mark.parametrize("call", WHERE, indirect=True)
+@pytest.mark.parametrize("slope", [0.05, 0.5, -0.5])
+def test_logits_that_climb_from_tile_to_tile(call, slope):
+    """Every tile of the vocabulary lies above (below) the one before, by less and by more than a tile may add before the reference moves."""
+    x = make(70, 3000, 64, seed=76)
+    x["b"] = slope * torch.arange(3000, dtype=torch.float32)
+    close(call(x), expect(x), f"slope {slope}")
+    for topk in (0, 3):
+        y = confident(0.0, topk, vocab=3000)
+        y["b"] = torch.arange(3000).div(128, rounding_mode="floor") * (1.0 / 64)
+        close(call(y, reduction="sum"), expect_confident(y), "confident")
