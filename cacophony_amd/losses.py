@@ -61,7 +61,7 @@ class _Head:
             raise ValueError(f"{what}: expected hidden [..., dim] and weight [vocab, dim], got {tuple(hidden.shape)} and {tuple(weight.shape)}")
         if bias is not None and tuple(bias.shape) != (weight.shape[0],):
             raise ValueError(f"{what}: bias must be [{weight.shape[0]}], got {tuple(bias.shape)}")
-        self.what, self.reduction = what, _REDUCTIONS[reduction]
+        self.what, self.reduction_name, self.reduction = what, reduction, _REDUCTIONS[reduction]
         self.vocab, self.dim = int(weight.shape[0]), int(weight.shape[1])
         self.lead = tuple(hidden.shape[:-1])
         self.hidden, self.ld_h = _rows(hidden.detach().reshape(-1, self.dim))
@@ -146,24 +146,28 @@ class _LinearLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, head, target, ignore_index, piece_bytes):
         out, lse = _forward(head, target, ignore_index, True)
-        # the tensors themselves (a detached one shares their version): a change in place before the backward pass is an error
-        ctx.save_for_backward(hidden, weight, bias, *(t for t in target.values() if torch.is_tensor(t)))
-        ctx.head, ctx.target, ctx.lse, ctx.ignore_index, ctx.piece_bytes = head, target, lse, ignore_index, piece_bytes
+        # All tensors that the backward pass reads are saved here and nowhere else: a change in place is an error (a detached tensor shares its
+        # version), hooks on saved tensors see them, and they are free once the backward pass is over.
+        names = tuple(k for k, t in target.items() if torch.is_tensor(t))
+        ctx.save_for_backward(hidden, weight, bias, lse, *(target[k] for k in names))
+        ctx.names, ctx.rest = names, {k: v for k, v in target.items() if k not in names}
+        ctx.what, ctx.reduction, ctx.ignore_index, ctx.piece_bytes = head.what, head.reduction_name, ignore_index, piece_bytes
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        hidden, weight, bias = ctx.saved_tensors[:3]
-        head = ctx.head
-        with torch.cuda.device(head.device):
+        with torch.cuda.device(grad.device):
             if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError(f"{head.what}: the autograd form cannot be captured into a graph; capture {head.what}_with_grad")
+                raise RuntimeError(f"{ctx.what}: the autograd form cannot be captured into a graph; capture {ctx.what}_with_grad")
+            hidden, weight, bias, lse, *tensors = ctx.saved_tensors
+            head = _Head(ctx.what, hidden, weight, bias, ctx.reduction)
+            target = {**dict(zip(ctx.names, tensors)), **ctx.rest}
             new = lambda n, t: torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and ctx.needs_input_grad[n] else None
             dh, dw, db = new(0, hidden), new(1, weight), new(2, bias)
             grad = grad.to(torch.float32).contiguous()
             kw = {"grad_scale": grad} if head.reduction else {"row_weight": grad.reshape(-1)}
-            _call(head, ctx.target, BACKWARD | LSE_PAIR, ignore_index=ctx.ignore_index, lse=ctx.lse, d_hidden=dh, d_weight=dw, d_bias=db,
+            _call(head, target, BACKWARD | LSE_PAIR, ignore_index=ctx.ignore_index, lse=lse, d_hidden=dh, d_weight=dw, d_bias=db,
                   piece_bytes=ctx.piece_bytes, **kw)
         return dh, dw, db, None, None, None, None
 

@@ -218,3 +218,66 @@ def test_logits_that_climb_from_tile_to_tile(call, slope):
         y = confident(0.0, topk, vocab=3000)
         y["b"] = torch.arange(3000).div(128, rounding_mode="floor") * (1.0 / 64)
         close(call(y, reduction="sum"), expect_confident(y), "confident")
+
+
+# ------------------------------------------------------------------------------------------------------------------------------------
+# autograd: what the backward pass holds
+# ------------------------------------------------------------------------------------------------------------------------------------
+def leaves(x):
+    d = dev(x)
+    for k in ("h", "w", "b"):
+        d[k] = d[k].clone().requires_grad_(True)
+    return d
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("topk", [0, 6])
+def test_saved_tensor_hooks_are_what_the_backward_pass_reads(topk):
+    """Hooks that keep copies on the host: the gradients are the same bits.  Hooks that hand back other hidden states: the gradients are another's."""
+    x = make(70, 400, 64, topk=topk, seed=77)
+    plain = leaves(x)
+    loss_of(plain).backward()
+    packed = []
+
+    def pack(t):
+        packed.append(t.shape)
+        return t.cpu()
+    d = leaves(x)
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.cuda()):
+        loss = loss_of(d)
+    assert {tuple(d[k].shape) for k in ("h", "w", "b")} <= {tuple(s) for s in packed}
+    loss.backward()
+    for k in ("h", "w", "b"):
+        assert torch.equal(d[k].grad, plain[k].grad)
+    d = leaves(x)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: torch.zeros_like(t) if t.shape == d["h"].shape else t):
+        loss = loss_of(d)
+    loss.backward()
+    assert not d["w"].grad.any() and d["b"].grad.any()      # d weight = dz^T . hidden
+
+
+@pytest.mark.gpu
+def test_saved_tensors_are_free_after_the_backward_pass():
+    """Hidden states that only the loss's graph holds: 4 MiB, free once the backward pass is over, though the loss itself is still there."""
+    d = dev(make(4096, 100, 512, seed=78))
+    one = torch.ones((), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    middle = d["h"] * one
+    loss = loss_of(dict(d, h=middle))
+    nbytes = middle.untyped_storage().nbytes()
+    del middle
+    held = torch.cuda.memory_allocated()
+    loss.backward()
+    assert one.grad is not None and nbytes == 4 << 20 and held - torch.cuda.memory_allocated() >= nbytes
+    with pytest.raises(RuntimeError, match="second time"):
+        loss.backward()
+
+
+@pytest.mark.gpu
+def test_backward_pass_twice():
+    d = leaves(make(70, 400, 64, topk=4, seed=79))
+    loss = loss_of(d, reduction="sum")
+    loss.backward(retain_graph=True)
+    first = {k: d[k].grad.clone() for k in ("h", "w", "b")}
+    loss.backward()
+    for k, g in first.items():
+        assert torch.equal(d[k].grad, g + g)
