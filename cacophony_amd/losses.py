@@ -8,7 +8,7 @@ taken in pieces of the vocabulary.
 
 Two forms of each loss:
 
-* `linear_cross_entropy` / `linear_topk_distillation` take part in autograd.
+* `linear_cross_entropy` / `linear_topk_distillation` take part in autograd, in reverse mode: tensors with a tangent are refused.
 * `..._with_grad` return the loss and the gradients of one call: one preparation for both passes, no autograd state, and they may be
   captured into a graph.  (The autograd forms refuse to be captured with gradients on: a captured backward pass whose leaves still have
   an eager graph alive would wait for that graph's stream inside the capture.)
@@ -22,6 +22,7 @@ import ctypes as C
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -172,6 +173,12 @@ class _LinearLoss(torch.autograd.Function):
         return dh, dw, db, None, None, None, None
 
 
+def _reverse_mode_only(what: str, *tensors) -> None:
+    for t in tensors:
+        if torch.is_tensor(t) and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what}: there is no forward-mode derivative; a tangent would be lost")
+
+
 def _loss(head: _Head, target: dict, hidden, weight, bias, ignore_index: int, piece_bytes: int) -> Tensor:
     if int(piece_bytes) <= 0:
         raise ValueError(f"{head.what}: piece_bytes must be positive, got {piece_bytes}")
@@ -203,6 +210,7 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, labels: Tensor, bias: O
     """logsumexp(z) - z[label] with z = hidden @ weight.T + bias, fp32.  A row whose label is `ignore_index` or outside [0, vocab) has
     loss 0 and does not count for the mean (which is NaN, with zero gradients, when no row does).  reduction "none" gives the rows'
     losses - minus the log-likelihood of each token - in the shape of `labels`."""
+    _reverse_mode_only("linear_cross_entropy", hidden, weight, bias)
     head = _Head("linear_cross_entropy", hidden, weight, bias, reduction)
     return _loss(head, _labels(head, labels), hidden, weight, bias, ignore_index, piece_bytes)
 
@@ -220,7 +228,8 @@ def linear_topk_distillation(hidden: Tensor, weight: Tensor, teacher_logits: Ten
     """T^2 KL(q || softmax(z / T)) with z = hidden @ weight.T + bias and q = softmax(teacher_logits / T) over the entries a teacher gives
     per row: teacher_logits [..., k], teacher_indices int32 or int64 [..., k], k <= 128 (`retrieval.topk` or `torch.topk` of the teacher's
     logits).  An index outside [0, vocab) (`retrieval.topk` pads with -1) or a logit of -inf is no entry, entries of one token add up, a
-    row without entries has loss 0 and does not count.  temperature 2^-20 .. 2^20."""
+    row without entries has loss 0 and does not count.  No gradient flows to the teacher.  temperature 2^-20 .. 2^20."""
+    _reverse_mode_only("linear_topk_distillation", hidden, weight, bias)
     head = _Head("linear_topk_distillation", hidden, weight, bias, reduction)
     return _loss(head, _teacher(head, teacher_logits, teacher_indices, temperature), hidden, weight, bias, -100, piece_bytes)
 

@@ -281,3 +281,29 @@ def test_backward_pass_twice():
     loss.backward()
     for k, g in first.items():
         assert torch.equal(d[k].grad, g + g)
+
+
+# ------------------------------------------------------------------------------------------------------------------------------------
+# refusals
+# ------------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("name", ["h", "w", "b"])
+@pytest.mark.parametrize("topk", [0, 3])
+def test_forward_mode_is_refused(topk, name):
+    """A tangent has nowhere to go; without the refusal it would be dropped where nothing requires a gradient."""
+    import torch.autograd.forward_ad as fwd
+    x = make(4, 20, 8, topk=topk, seed=80)
+    with fwd.dual_level():
+        y = dict(x, **{name: fwd.make_dual(x[name], torch.ones_like(x[name]))})
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            loss_of(y)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            loss_of(y)
+
+
+@pytest.mark.gpu
+def test_inside_a_dual_level_plain_tensors_are_taken():
+    import torch.autograd.forward_ad as fwd
+    x = make(20, 100, 64, seed=81)
+    with fwd.dual_level():
+        got = loss_of(dev(x))
+    assert torch.equal(got, loss_of(dev(x)))
