@@ -19,6 +19,7 @@ dimensions.  dim is a multiple of 8.  Any strides are taken; rows that do not st
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -51,11 +52,11 @@ class _Head:
     def __init__(self, what: str, hidden: Tensor, weight: Tensor, bias: Optional[Tensor], reduction: str):
         if reduction not in _REDUCTIONS:
             raise ValueError(f"{what}: reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
-        for name, t, dt in (("hidden", hidden, torch.bfloat16), ("weight", weight, torch.bfloat16), ("bias", bias, torch.float32)):
-            if t is None:
-                continue
+        operands = [("hidden", hidden, torch.bfloat16), ("weight", weight, torch.bfloat16)] + ([] if bias is None else [("bias", bias, torch.float32)])
+        for name, t, dt in operands:
             if not torch.is_tensor(t) or t.dtype != dt:
                 raise ValueError(f"{what}: {name} must be a {dt} tensor, got {t.dtype if torch.is_tensor(t) else type(t)}")
+        for name, t, _ in operands:
             if t.device.type != "cuda" or t.device != hidden.device:
                 raise RuntimeError(f"{what}: hidden, weight and bias must be on the same GPU, {name} is on {t.device}")
         if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]:
@@ -65,7 +66,7 @@ class _Head:
         self.what, self.reduction_name, self.reduction = what, reduction, _REDUCTIONS[reduction]
         self.vocab, self.dim = int(weight.shape[0]), int(weight.shape[1])
         self.lead = tuple(hidden.shape[:-1])
-        self.hidden, self.ld_h = _rows(hidden.detach().reshape(-1, self.dim))
+        self.hidden, self.ld_h = _rows(hidden.detach().reshape(math.prod(self.lead), self.dim))
         self.weight, self.ld_w = _rows(weight.detach())
         self.bias = None if bias is None else bias.detach().contiguous()
         self.rows = int(self.hidden.shape[0])

@@ -307,3 +307,20 @@ def test_inside_a_dual_level_plain_tensors_are_taken():
     with fwd.dual_level():
         got = loss_of(dev(x))
     assert torch.equal(got, loss_of(dev(x)))
+
+
+@pytest.mark.parametrize("change", [dict(h=None), dict(w=None), dict(h="states"), dict(w=torch.zeros(20, 8)), dict(b=torch.zeros(20).double())])
+def test_operands_that_are_no_tensors_or_of_another_type(change):
+    """Types are looked at before devices: the message names what is wrong wherever the rest lies."""
+    x = dict(make(4, 20, 8, seed=82), **change)
+    with pytest.raises(ValueError, match="|".join({"h": "hidden", "w": "weight", "b": "bias"}[k] for k in change)):
+        loss_of(x)
+
+
+@pytest.mark.gpu
+def test_empty_dimensions_are_refused():
+    for shape_h, shape_w in (((4, 0), (20, 0)), ((4, 8), (0, 8)), ((2, 0, 0), (20, 0))):
+        h, w = torch.zeros(shape_h, dtype=torch.bfloat16, device="cuda"), torch.zeros(shape_w, dtype=torch.bfloat16, device="cuda")
+        y = torch.zeros(shape_h[:-1], dtype=torch.long, device="cuda")
+        with pytest.raises(ValueError):
+            loss_of(dict(h=h, w=w, y=y, b=None, topk=0))
