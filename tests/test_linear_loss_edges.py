@@ -324,3 +324,62 @@ def test_empty_dimensions_are_refused():
         y = torch.zeros(shape_h[:-1], dtype=torch.long, device="cuda")
         with pytest.raises(ValueError):
             loss_of(dict(h=h, w=w, y=y, b=None, topk=0))
+
+
+# ------------------------------------------------------------------------------------------------------------------------------------
+# the paths of the large calls against 64 bits
+# ------------------------------------------------------------------------------------------------------------------------------------
+def expect_on_gpu(d, *args, **kw):
+    """`expect` for operands on the GPU, computed there in 64 bits."""
+    with torch.device("cuda"):
+        out = expect(d, *args, **kw)
+    return {k: tuple(t.cpu() for t in v) for k, v in out.items()}
+
+
+def test_simulator_transposed_weights(sim):
+    """2048 rows and more read the weights transposed; with two column blocks, off the tiles in every direction, in one piece and in five."""
+    x = make(2304, 1100, 264, seed=90)
+    want = expect(x)
+    close(sim_call(x), want, "one piece")
+    close(sim_call(x, piece=1), want, "pieces")
+
+
+# d hidden is shared out in whole tiles per workgroup (32 tiles and more) next to a list, and in 8, 4, 2 or 1 slices of the vocabulary (from 32, 64, 128, 256
+# tiles of 256 x 256 on); 2048 rows and more read transposed weights, fewer do not
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,dim,topk,T,bias,ignored", [
+    (2304, 4200, 264, 0, 1.0, True, 0.0), (2200, 5003, 1288, 0, 1.0, True, 0.0), (2600, 4999, 1544, 20, 2.0, True, 0.0), (1100, 3001, 4104, 0, 1.0, False, 0.0),
+    (1200, 2500, 7176, 5, 1.0, True, 0.0), (8192, 300, 2056, 0, 1.0, True, 0.0), (3500, 9001, 520, 40, 1.5, False, 0.3)])
+def test_large_calls(rows, vocab, dim, topk, T, bias, ignored):
+    d = dev(make(rows, vocab, dim, topk=topk, bias=bias, seed=rows, ignored=ignored))
+    want = expect_on_gpu(d, T)
+    close(with_grad(d, T)._asdict(), want, "one piece")
+    close(with_grad(d, T, piece_bytes=1)._asdict(), want, "pieces of one tile")
+    close(with_grad(d, T, piece_bytes=4 * 2048 * rows)._asdict(), want, "pieces of eight tiles")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("topk", [0, 32])
+def test_a_full_caption_head(topk):
+    """256 captions of 32 tokens, a third of them padding, on the caption decoder's head: the whole vocabulary in one piece, and in nine."""
+    d = dev(make(8192, 50265, 768, topk=topk, seed=91))
+    T = 2.0 if topk else 1.0
+    want = expect_on_gpu(d, T)
+    close(with_grad(d, T)._asdict(), want, "one piece")
+    close(with_grad(d, T, piece_bytes=192 << 20)._asdict(), want, "nine pieces")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,dim", [(700, 17000, 520), (2500, 6000, 776)])
+@pytest.mark.parametrize("topk", [0, 9])
+def test_autograd_of_large_calls_each_gradient_alone(rows, vocab, dim, topk):
+    """More than 128 of the large tiles, three column blocks, in several pieces; the weights as they lie and transposed."""
+    x = make(rows, vocab, dim, topk=topk, seed=92)
+    want = expect_on_gpu(dev(x))
+    names = {"h": "d_hidden", "w": "d_weight", "b": "d_bias"}
+    for some in (("h",), ("w",), ("b",), ("w", "b"), ("h", "w", "b")):
+        d = dev(x)
+        for k in some:
+            d[k].requires_grad_(True)
+        got = torch.autograd.grad(loss_of(d, piece_bytes=4 * 2048 * rows), [d[k] for k in some])
+        close({names[k]: g for k, g in zip(some, got)}, want, str(some))
