@@ -150,3 +150,28 @@ def test_nll_on_another_stream_and_after_other_work(model, clips):
     side.synchronize()
     assert torch.equal(got, want)
     assert (large[:2] - large[38:]).abs().max() < 1e-4
+
+
+@pytest.mark.gpu
+def test_nll_against_the_references_logits_token_by_token(model, clips):
+    """The logits' bar of rel-L2 1e-2 spread over a row's V logits is 1e-2 rms(z) for each.  The errors come from bf16 roundings of operands and states, many
+    and independent, so a label's is within five times that for every one of the scored tokens (5 sigma: 6e-7 of a normal distribution), the error of
+    logsumexp, a mean over the words, well within the same, and the mean over n tokens within 5 / sqrt(n) of it.  What the bound is worth: likelihoods of
+    other words - the label 17 words on, the token before instead of the one after, a constant - are outside it for most tokens."""
+    g = load_golden("decoder_tiny.npz")
+    ab, ah = clips
+    nll = model.get_caption_nll(ah, ab["audio_mask"], g["ids"], g["tmask"]).cpu().double()
+    z, V = torch.from_numpy(g["logits"][:, :-1]).double(), g["logits"].shape[-1]
+    ids, scored = torch.as_tensor(g["ids"]).long(), torch.as_tensor(g["tmask"])[:, 1:] != 0
+    lp = torch.log_softmax(z, -1)
+    bound = 5e-2 * z.square().mean(-1).sqrt()
+
+    def inside(label):
+        return ((nll + lp.gather(2, label[..., None])[..., 0]).abs() <= bound)[scored]
+    n = int(scored.sum())
+    assert n > 40 and inside(ids[:, 1:]).all()
+    err = (nll + lp.gather(2, ids[:, 1:, None])[..., 0])[scored]
+    assert abs(err.mean()) <= bound[scored].mean() / n ** 0.5
+    for label in ((ids[:, 1:] + 17) % V, ids[:, :-1]):
+        assert inside(label).double().mean() < 0.15
+    assert ((nll - float(np.log(V))).abs() <= bound)[scored].double().mean() < 0.15
