@@ -37,18 +37,27 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int MAX_WG = 512;          // most workgroups of a persistent launch (two per CU)
 constexpr int MAX_CU = 256;
-// From this many rows on d hidden reads transposed weights.  Transposing costs 4 bytes of traffic per weight, whatever the rows; it saves 0.65 us
-// per K-tile and workgroup, which pays from about 1300 rows on (768 x 50265: 35 us against 130 us at 5489 rows, 30 at 1187).
+// From this many rows on d hidden reads transposed weights.  Transposing costs 4 bytes of traffic per weight, whatever the rows, and saves its share of every
+// K-tile.  Calls with gradients, us as the weights lie / transposed, rows x (vocabulary x dim):
+//            50265 x 768    32007 x 520    10000 x 2048    20000 x 4096
+//   1187      444 / 471      298 / 298      250 / 269       775 / 805
+//   1800      681 / 719      400 / 389      388 / 392      1081 / 1101
+//   2304      745 / 764      480 / 471      444 / 454      1299 / 1285
+//   4096     1270 / 1227     732 / 703      657 / 659      2115 / 2044
+//   8192     2389 / 2271    1375 / 1300    1188 / 1149     4216 / 4004
+// The two meet between 1200 and 4100 rows, another number for every head; at 2048 the choice is within 3 % of the better one for all of these.
 constexpr int WT_ROWS = 2048;
 
 typedef VgTile<8, 4, 2, 4> Big;      // 256 x 256, one workgroup per CU
 typedef VgTile<4, 2, 1, 4> Small;    // 64 x 128, two per CU: for calls that read the weights and do little else
-// Up to this many rows take Small.  768 x 50265: lse for one token 18 us (4.3 TB/s), with Big 30; a call with gradients for 65 / 128 rows 135 / 143 us, with
-// Big 143 / 150 (520 x 32007: 106 / 110, with Big 121 / 125).  From 129 rows on Big is as fast or faster (149 rows: 154 us, with Small 173).
+// Up to this many rows take Small.  With gradients, 768 x 50265: 65 / 128 rows 135 / 143 us, with Big 143 / 150 (520 x 32007: 106 / 110, 121 / 125); from 129
+// rows on Big is as fast or faster (149 rows: 154 us, with Small 173).  Losses alone, 768 x 50265: one token's logits 18 us (4.3 TB/s), with Big 30; whole
+// calls for 65 / 128 / 129 / 256 rows 37 / 37 / 46 / 44 us, with Big 39 / 38 / 38 / 39.  (A head as large as 4096 x 131072 changes over earlier: 32 / 65 / 128
+// rows 187 / 250 / 251, with Big 231 / 228 / 233.)
 constexpr int SMALL_ROWS = 128;
 // ... and so do calls that would have at most this many of Big's tiles, which would leave half the CUs idle.  Calls with gradients, us, rows x
 // vocabulary x dim: 24 tiles (700 x 2000 x 2048) 94, with Big 147; 48 (300 x 6000 x 512) 63, 84; 118 (300 x 15000 x 512) 102, 107; 160 (1000 x 10000 x 512)
-// 119, 114; 236 (300 x 30000 x 1000) 208, 197.
+// 119, 114; 236 (300 x 30000 x 1000) 208, 197.  Losses alone on 20000 x 2048: 79 tiles (128 / 256 rows) 36 / 48, with Big 56 / 56; 158 (300 rows) 64, 58.
 constexpr int SMALL_TILES = 128;
 
 // what the kernels share; device pointers into the caller's tensors or the workspace
@@ -490,7 +499,7 @@ __device__ __forceinline__ void lse_body(const LossArgs& a, char* smem) {
   float nref[C::MI], sm[C::MI];      // minus the reference, the sum
 #pragma unroll
   for (int q = 0; q < C::MI; ++q) { nref[q] = 3.0e38f; sm[q] = 0.f; }
-  vg_run<C, false, false, true, true, true>(
+  vg_run<C, false, true, true, true>(
       tiles, smem,
       [&](int, int& k0, int& k1) { k0 = 0; k1 = a.hp / VG_K; },
       [&](int) { return VgOperand{a.hc + (int64_t)L.rb * C::BM * a.hp, a.hp, C::BM, a.hp, 0}; },      // of the tile whose weights were asked for before
@@ -753,7 +762,7 @@ __device__ __forceinline__ void dlogits_body(const LossArgs& a, char* smem) {
   if (tiles == 0) return;
   const float cs = a.inv_t * LOG2E;
   const bool label = !a.topk;
-  vg_run<C, false, false, true, true, true>(
+  vg_run<C, false, true, true, true>(
       tiles, smem,
       [&](int, int& k0, int& k1) { k0 = 0; k1 = a.hp / VG_K; },
       [&](int) { return VgOperand{a.hc + (int64_t)L.rb * C::BM * a.hp, a.hp, C::BM, a.hp, 0}; },      // of the tile whose weights were asked for before
@@ -868,8 +877,9 @@ __global__ __launch_bounds__(256) void targets2_kernel(LossArgs a) {
 // How a piece's gradient work is shared out, XCD by XCD.
 //   d weight   an XCD takes a run of whole tiles, its workgroups one after the other, column blocks fastest: they share a panel of d logits.
 //   d hidden   `ks` slices of the vocabulary times 8 / ks runs of the output tiles: the fewest slices that leave an XCD a tile for each of its
-//              workgroups, so that these walk the same part of the vocabulary together, with few panels between them (at 22 row blocks and
-//              3 column blocks 0.4 MB per K-tile instead of 2 MB, which the XCD's L2 then holds).  Tiles beyond a multiple of the
+//              workgroups, so that these walk the same part of the vocabulary together, with few panels between them: at 22 row blocks and
+//              3 column blocks the launch takes 1.8 GB through the L2s, which hold 72 % of what it reads, and 653 us; with one
+//              slice 4.0 GB, 41 % and 768 us.  Tiles beyond a multiple of the
 //              workgroups make one list of K-tiles, cut so that workgroups with one d weight tile less get more of it.
 // A slice of a whole tile is kept at [tile][slice], a part of the list at [XCD][tile of the list + workgroup] (the sum grows from part to
 // part, so the places are distinct).
@@ -934,7 +944,7 @@ __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
   const Share S(a, n, gridDim.x, xcd);
   // d weight: both operands with the token fastest
   if (slot < S.wcnt)
-    vg_run<C, false, false, false, false, false>(
+    vg_run<C, false, false, false, false>(
         (S.wcnt - slot + S.slots - 1) / S.slots, smem,
         [&](int i, int& k0, int& k1) {
           const int run = (S.wbase + slot + i * S.slots) & ((1 << a.lw) - 1);
@@ -981,7 +991,7 @@ __device__ __forceinline__ void grads_body(const LossArgs& a, char* smem) {
   if (parts == 0) return;
   const bool first_piece = a.v0 == 0;
   auto out_tile = [&](int i) { return i < S.whole ? S.t0 + slot + i * S.slots : S.t0 + S.whole * S.slots + l0 + i - S.whole; };
-  vg_run<C, false, !WT, false, false, false>(
+  vg_run<C, !WT, false, false, false>(
       parts, smem,
       [&](int i, int& k0, int& k1) {
         const int at = i < S.whole ? 0 : (l0 + i - S.whole) * S.nkx;      // the tile's first K-tile in the list

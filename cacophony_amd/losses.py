@@ -2,9 +2,11 @@
 a teacher's top logits.  C ABI: caco_linear_ce / caco_linear_distill (include/caco_hip.h has the formulas).
 
 The reference forms the logits [tokens, vocab] of its caption decoder (`decoder_proj`, src/caco_torch/text_models/roberta.py:371,
-src/caco_torch/caco.py:212-240) and leaves what follows to its callers; at 256 captions of 32 tokens that matrix alone is 1.6 GB.
-Here the rows' losses come out of the same pass that forms a tile of logits, and the gradients of hidden states, weight and bias are
-taken in pieces of the vocabulary.
+src/caco_torch/caco.py:212-240) and leaves what follows to its callers; at 256 captions of 32 tokens that matrix alone is 1.6 GB in fp32.
+Here the rows' losses come out of the same pass that forms a tile of logits: losses alone take 16 MB at that size.  The gradients
+of hidden states, weight and bias go through the gradient of the logits, in bf16 and for one piece of the vocabulary at a time, and
+`piece_bytes` is what it may take: by default 2 GiB, which is the whole vocabulary at that size (1.59 ms, a workspace of 2.0 GB).
+Smaller pieces trade time for memory: 1.85 ms in 750 MB (512 MiB of pieces), 3.2 in 450 (128), 8.4 in 346 (32).
 
 Two forms of each loss:
 
@@ -33,7 +35,7 @@ Tensor = torch.Tensor
 
 FORWARD, BACKWARD, LSE_PAIR = 1, 2, 4
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
-# d logits of one piece of the vocabulary, bf16, by rows and by columns: 8192 tokens x 50265 words are one piece, 0.6 % of a card's memory
+# d logits of one piece of the vocabulary, bf16, by rows and by columns: 8192 tokens x 50265 words are one piece, with the rest 0.7 % of a card's memory
 PIECE_BYTES = 2 << 30
 
 
@@ -191,7 +193,7 @@ def _loss(head: _Head, target: dict, hidden, weight, bias, ignore_index: int, pi
     return _forward(head, target, ignore_index, False)[0]
 
 
-def _with_grad(head: _Head, target: dict, weight: Tensor, ignore_index: int, row_weight: Optional[Tensor], piece_bytes: int) -> LinearLossGrads:
+def _with_grad(head: _Head, target: dict, ignore_index: int, row_weight: Optional[Tensor], piece_bytes: int) -> LinearLossGrads:
     if row_weight is not None:
         row_weight = head.per_row("row_weight", row_weight)
         if row_weight.dtype != torch.float32:
@@ -221,7 +223,7 @@ def linear_cross_entropy_with_grad(hidden: Tensor, weight: Tensor, labels: Tenso
     """The loss, the rows' losses and the gradients of sum(row_weight * row_loss), for "mean" divided by the number of rows that
     count.  row_weight fp32 in the shape of `labels`, None = 1."""
     head = _Head("linear_cross_entropy", hidden, weight, bias, reduction)
-    return _with_grad(head, _labels(head, labels), weight, ignore_index, row_weight, piece_bytes)
+    return _with_grad(head, _labels(head, labels), ignore_index, row_weight, piece_bytes)
 
 
 def linear_topk_distillation(hidden: Tensor, weight: Tensor, teacher_logits: Tensor, teacher_indices: Tensor, bias: Optional[Tensor] = None, *,
@@ -240,4 +242,4 @@ def linear_topk_distillation_with_grad(hidden: Tensor, weight: Tensor, teacher_l
                                        piece_bytes: int = PIECE_BYTES) -> LinearLossGrads:
     """The distillation loss with its gradients in one call; see `linear_cross_entropy_with_grad`.  No gradient flows to the teacher."""
     head = _Head("linear_topk_distillation", hidden, weight, bias, reduction)
-    return _with_grad(head, _teacher(head, teacher_logits, teacher_indices, temperature), weight, -100, row_weight, piece_bytes)
+    return _with_grad(head, _teacher(head, teacher_logits, teacher_indices, temperature), -100, row_weight, piece_bytes)

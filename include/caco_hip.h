@@ -178,7 +178,7 @@ int caco_decoder_forward(caco_model* m, const float* text_hidden_dev, const int6
 
 /* ... and the likelihoods of given tokens instead of the logits: nll_dev fp32 [B, T] = -log softmax(logits[b, t])[targets[b, t]], 0 where
  * targets_dev int64 [B, T] is ignore_index or outside the vocabulary.  The reference has the logits only (caco.py:212-240); scoring 256
- * captions of 32 tokens through them takes 3.3 GB for the logits (scratch and output), this call 18 MB in their place. */
+ * captions of 32 tokens through them takes 3.3 GB for the logits (scratch and output), this call 16 MB in their place. */
 int caco_decoder_score(caco_model* m, const float* text_hidden_dev, const int64_t* text_mask_dev, const float* audio_hidden_dev,
                        const float* audio_mask_dev, const int64_t* targets_dev, int64_t ignore_index, int32_t batch, int32_t seq_text,
                        int32_t seq_audio, float* nll_dev, void* stream);
@@ -226,7 +226,8 @@ void caco_decode_end(caco_decode_state* s);
  *   (0 is allowed), vocab <= 2^24, rows * vocab <= 2^46 (both rounded up to 256), dim <= 65536.
  * ws_dev: scratch of the caller's, 16-byte aligned, its contents are not kept; one call at a time may use it.  caco_linear_loss_workspace
  *   gives its size (topk 0 = cross entropy; < 0: CACO_ERR_INVALID); with the backward pass it includes the gradient of the logits
- *   for one piece of the vocabulary in bf16, twice, of about piece_bytes together (at least 256 columns).  A smaller workspace makes more pieces.
+ *   for one piece of the vocabulary in bf16, twice, of about piece_bytes together (at least 256 columns).  A smaller workspace makes more pieces: 8192 x 50265 x
+ *   768 with gradients 1.59 ms in one piece and 2.0 GB, 1.85 in 750 MB, 3.2 in 450, 8.4 in 346, 31 in 319 (a tile's columns a piece); forward alone 16 MB.
  * Capturable into a graph: no synchronisation, no allocation, no memset; equal calls give equal bits. */
 #define CACO_LOSS_FORWARD 1
 #define CACO_LOSS_BACKWARD 2
