@@ -89,6 +89,7 @@ _SIGNATURES = {
     "caco_decode_step": (C.c_int, [_vp, _vp, _vp, _vp]),
     "caco_decode_end": (None, [_vp]),
     "caco_decoder_forward": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp]),
+    "caco_decoder_hidden": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp]),
     "caco_decoder_score": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp]),
 }
 

@@ -1078,6 +1078,20 @@ int caco_decoder_forward(caco_model* m, const float* text_hidden, const int64_t*
   return CACO_OK;
 }
 
+// The same up to what the projection takes (decoder_proj, roberta.py:371): the states on which a head is trained or distilled.
+int caco_decoder_hidden(caco_model* m, const float* text_hidden, const int64_t* text_mask, const float* audio_hidden, const float* audio_mask,
+                        int32_t batch, int32_t seq_t, int32_t seq_a, void* hidden, void* stream) {
+  CACO_TRY(check_decoder(m, text_hidden, text_mask, audio_hidden, audio_mask, hidden, batch, seq_t, seq_a, "caco_decoder_hidden"));
+  hipStream_t st = (hipStream_t)stream;
+  const int64_t M = (int64_t)batch * seq_t, Ma = (int64_t)batch * seq_a;
+  Arena A(m, WS_TEXT, st);
+  const DecoderWs w(A, M, Ma, m->cfg.text_hidden, m->cfg.text_intermediate);
+  CACO_TRY(A.commit(st));
+  CACO_TRY(run_decoder(m, A, w, text_hidden, text_mask, audio_hidden, audio_mask, batch, seq_t, seq_a, st));
+  CACO_HIP(hipMemcpyAsync(hidden, A.at<bf16_t>(w.xb), (size_t)M * m->cfg.text_hidden * 2, hipMemcpyDeviceToDevice, st));
+  return CACO_OK;
+}
+
 // The same up to the likelihoods of given tokens: the vocabulary's logits exist a tile at a time only (linear_loss.hip).
 int caco_decoder_score(caco_model* m, const float* text_hidden, const int64_t* text_mask, const float* audio_hidden, const float* audio_mask,
                        const int64_t* targets, int64_t ignore_index, int32_t batch, int32_t seq_t, int32_t seq_a, float* nll, void* stream) {

@@ -260,6 +260,20 @@ class CACO(_HipModel):
                                                        deterministic=deterministic)
         return self._decoder_forward(text_hidden_state, text_mask, audio_hidden_state, audio_mask, deterministic)
 
+    def get_decoder_hidden_state(self, audio_hidden_state, audio_mask, text_input_ids, text_mask, deterministic: bool = True) -> Tensor:
+        """What `get_decoder_logits` projects to the vocabulary (decoder_proj, text_models/roberta.py:371), bf16 [B, T, hidden]: the hidden states for
+        `losses.linear_cross_entropy` / `linear_topk_distillation`, with `decoder_module.decoder_proj` of the state dict as the head to train
+        (bf16 weight, fp32 bias).  C ABI: caco_decoder_hidden."""
+        if self.decoder_module is None:
+            raise ValueError("Decoder module not initialized")      # caco.py:223-224
+        _, text_hidden_state = self.get_text_embedding(text_input_ids=text_input_ids, text_mask=text_mask, deterministic=deterministic)
+        th, tm, ah, am, B, T, S = self._decoder_operands(text_hidden_state, text_mask, audio_hidden_state, audio_mask)
+        hidden = torch.empty(B, T, self.text_config.hidden_size, dtype=torch.bfloat16, device=self.device)
+        with torch.cuda.device(self.device):
+            _lib.check(self._lib.caco_decoder_hidden(self._handle, _ptr(th), _ptr(tm), _ptr(ah), _ptr(am), B, T, S, _ptr(hidden), _stream()),
+                       "decoder")
+        return hidden
+
     def get_caption_nll(self, audio_hidden_state, audio_mask, text_input_ids, text_mask, deterministic: bool = True) -> Tensor:
         """-log p(token t + 1 | tokens 0 .. t, audio) of given captions, fp32 [B, T - 1]: the cross entropy of
         `get_decoder_logits(...)[:, :-1]` with `text_input_ids[:, 1:]`, 0 where text_mask[:, 1:] is 0.  The logits are not formed

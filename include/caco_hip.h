@@ -176,6 +176,11 @@ int caco_decoder_forward(caco_model* m, const float* text_hidden_dev, const int6
                          const float* audio_hidden_dev, const float* audio_mask_dev, int32_t batch, int32_t seq_text,
                          int32_t seq_audio, float* logits_dev, void* stream);
 
+/* ... and the last hidden states instead of the logits, hidden_dev bf16 [B, T, H]: what the projection takes (decoder_proj, roberta.py:371), and what caco_linear_ce /
+ * caco_linear_distill take to train a head or to distil it. */
+int caco_decoder_hidden(caco_model* m, const float* text_hidden_dev, const int64_t* text_mask_dev, const float* audio_hidden_dev,
+                        const float* audio_mask_dev, int32_t batch, int32_t seq_text, int32_t seq_audio, void* hidden_dev, void* stream);
+
 /* ... and the likelihoods of given tokens instead of the logits: nll_dev fp32 [B, T] = -log softmax(logits[b, t])[targets[b, t]], 0 where
  * targets_dev int64 [B, T] is ignore_index or outside the vocabulary.  The reference has the logits only (caco.py:212-240); scoring 256
  * captions of 32 tokens through them takes 3.3 GB for the logits (scratch and output), this call 16 MB in their place. */

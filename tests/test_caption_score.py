@@ -175,3 +175,77 @@ def test_nll_against_the_references_logits_token_by_token(model, clips):
     for label in ((ids[:, 1:] + 17) % V, ids[:, :-1]):
         assert inside(label).double().mean() < 0.15
     assert ((nll - float(np.log(V))).abs() <= bound)[scored].double().mean() < 0.15
+
+
+def test_hidden_states_refused_without_a_model():
+    lib = _lib.load()
+    one = C.c_void_p(1024)
+    assert lib.caco_decoder_hidden(None, one, one, one, one, 1, 1, 1, one, None) == _lib.CACO_ERR_INVALID
+
+
+@pytest.fixture(scope="module")
+def head(model):
+    a, t, cc, d = _configs()
+    state = synth.make_caco_state(a, t, cc, seed=0, decoder_cfg=d)
+    get = lambda n: torch.as_tensor(np.asarray(state["decoder_module.decoder_proj." + n])).float().cuda()
+    return get("weight").bfloat16(), get("bias")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,T", [(2, 24), (9, 1), (5, 33)])
+def test_hidden_states_are_what_the_head_projects(model, clips, head, n, T):
+    """The head on these states gives the decoder's logits (fp32 sums of the same products: 1e-3, as above), and the cross entropy on them the bits of
+    `get_caption_nll`, which does the same inside."""
+    from cacophony_amd import losses
+    ab, ah = clips
+    pick = torch.arange(n, device="cuda") % 2
+    ah, am = ah[pick], ab["audio_mask"][pick]
+    ids, mask = (torch.as_tensor(x).cuda() for x in synth.make_captions(n, T + 1, model.text_config.vocab_size, start=5))
+    h = model.get_decoder_hidden_state(ah, am, ids[:, :-1], mask[:, :-1])
+    assert h.shape == (n, T, 768) and h.dtype == torch.bfloat16
+    w, b = head
+    logits = model.get_decoder_logits(ah, am, ids[:, :-1], mask[:, :-1])
+    assert (h.reshape(-1, 768).float() @ w.float().t() + b - logits.reshape(n * T, -1)).abs().max() < 1e-3
+    labels = torch.where(mask[:, 1:] != 0, ids[:, 1:], -100)
+    nll = losses.linear_cross_entropy(h, w, labels, b, reduction="none")
+    assert torch.equal(nll, model.get_caption_nll(ah, am, ids, mask))
+
+
+@pytest.mark.gpu
+def test_a_head_trained_and_distilled_on_the_decoder(model, clips, head):
+    """As it is used: the decoder's states, the old head's best logits as a teacher for a new one, the captions as labels; both gradients against 64 bits."""
+    from cacophony_amd import losses, retrieval
+    from tests.test_linear_loss import close, expect
+    ab, ah = clips
+    ids, mask = (torch.as_tensor(x).cuda() for x in synth.make_captions(2, 28, model.text_config.vocab_size, start=21))
+    args = ah, ab["audio_mask"], ids[:, :-1], mask[:, :-1]
+    h, (w, b) = model.get_decoder_hidden_state(*args), head
+    idx, val = retrieval.topk(model.get_decoder_logits(*args).reshape(54, -1), 16)
+    idx = torch.where((mask[:, 1:] != 0).reshape(-1, 1), idx, -1)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    new = (w.float() + 0.02 * torch.randn(w.shape, generator=gen, device="cuda")).bfloat16().requires_grad_(True)
+    bias = torch.zeros_like(b, requires_grad=True)
+    x = dict(h=h.reshape(54, -1).cpu(), w=new.detach().cpu(), b=bias.detach().cpu())
+    loss = losses.linear_topk_distillation(h, new, val.reshape(2, 27, 16), idx.reshape(2, 27, 16), bias, temperature=2.0)
+    loss.backward()
+    close({"loss": loss, "d_weight": new.grad, "d_bias": bias.grad}, expect(dict(x, topk=16, teacher=val.cpu(), idx=idx.cpu().long()), 2.0), "distilled")
+    new.grad = bias.grad = None
+    labels = torch.where(mask[:, 1:] != 0, ids[:, 1:], -100)
+    loss = losses.linear_cross_entropy(h, new, labels, bias)
+    loss.backward()
+    close({"loss": loss, "d_weight": new.grad, "d_bias": bias.grad}, expect(dict(x, topk=0, y=labels.reshape(-1).cpu())), "trained")
+
+
+@pytest.mark.gpu
+def test_hidden_states_refusals(model, clips, tiny_state):
+    from cacophony_amd.model import CACO
+    a, t, cc, _ = _configs()
+    ab, ah = clips
+    ids = torch.zeros(2, 4, dtype=torch.long)
+    plain = CACO(a, t, cc, device="cuda:0").load_state_dict(tiny_state)
+    with pytest.raises(ValueError, match="Decoder module not initialized"):
+        plain.get_decoder_hidden_state(ah, ab["audio_mask"], ids, torch.ones_like(ids))
+    with pytest.raises(ValueError):
+        model.get_decoder_hidden_state(ah[:1], ab["audio_mask"][:1], ids, torch.ones_like(ids))
+    with pytest.raises((ValueError, IndexError)):
+        model.get_decoder_hidden_state(ah, ab["audio_mask"], ids + model.text_config.vocab_size, torch.ones_like(ids))
