@@ -32,7 +32,7 @@
 // Softmax statistics are fp32.  The exponent reference of a row is a LAZY running maximum of the raw scores: it only
 // moves when the row maximum outgrows it by more than 2^8 (softmax is invariant to the reference; P <= 256 meanwhile), so
 // the rescale of O runs about once per row block, not once per tile.  exp is exp2(fma(s, scale*log2e, -ref*scale*log2e)):
-// one packed FMA per two scores + one v_exp per score.  Mask work (key padding, causal diagonal) is only executed for
+// one FMA + one v_exp per score.  Mask work (key padding, causal diagonal) is only executed for
 // tiles that contain a masked key.
 // A query row whose keys are all masked yields 0 (the reference yields NaN there; it cannot happen with
 // right-padded inputs).
@@ -291,7 +291,7 @@ __device__ __forceinline__ void attention_body(const bf16_t* __restrict__ qp_, i
         }
         // Lazy exponent reference: softmax is invariant to the reference point, so m_run only moves when the row max
         // outgrows it by more than 2^8 (P <= 256 meanwhile; fp32 sums and bf16 P keep their relative precision).  The
-        // O rescale (24 packed multiplies per block) then runs about once per row block instead of once per tile.
+        // O rescale (48 multiplies per block) then runs about once per row block instead of once per tile.
         const bool grow = (m_tile - m_run[x]) * scale_log2 > 8.f;     // m_run = -inf: true unless the tile is all masked
         if (__ballot(grow) != 0ull) {
           const float m_new = grow ? m_tile : m_run[x];

@@ -124,7 +124,7 @@ __device__ __forceinline__ void w16_epilogue(const f32x4 (&acc)[8][4], const Gem
           }
           const f32x4 a = acc[i * 2 + ib][jb];
           bf16x4 o;
-          if constexpr (ACT == ACT_SILU) {   // packed pairs, see w8_epilogue
+          if constexpr (ACT == ACT_SILU) {   // in pairs, see w8_epilogue
             typedef float f32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
             for (int r = 0; r < 4; r += 2) {

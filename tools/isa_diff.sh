@@ -12,7 +12,7 @@ FILES=("$@")
 [ ${#FILES[@]} -eq 0 ] && FILES=(api gemm gemm_x gemm_w8 attention norm pool mel topk)
 OLD=$(mktemp -d) ; NEW=$(mktemp -d)
 git -C "$REPO" archive "$REF" cacophony_amd/csrc include | tar -x -C "$OLD"
-FLAGS="-O3 -std=c++17 --offload-arch=gfx950 -fno-gpu-rdc -ffp-contract=fast --cuda-device-only -S"
+FLAGS="-O3 -std=c++17 --offload-arch=gfx950 -fno-gpu-rdc -ffp-contract=fast -Xclang -target-feature -Xclang -packed-fp32-ops --cuda-device-only -S"
 rc=0
 for f in "${FILES[@]}"; do
   f=${f%.hip}

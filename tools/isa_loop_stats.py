@@ -14,7 +14,7 @@ src = sys.argv[1]
 filt = next((a for a in sys.argv[2:] if not a.startswith("-")), "")
 extra = [a for a in sys.argv[2:] if a.startswith("-")]
 path = src if os.path.exists(src) else os.path.join(REPO, "cacophony_amd", "csrc", src)
-asm = subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-fno-gpu-rdc", "-ffp-contract=fast",
+asm = subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-fno-gpu-rdc", "-ffp-contract=fast", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                       "--cuda-device-only", "-S", "-I", os.path.join(REPO, "include"), "-I", os.path.join(REPO, "cacophony_amd", "csrc"),
                       *extra, path, "-o", "-"], capture_output=True, text=True).stdout
 

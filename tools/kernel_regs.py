@@ -8,7 +8,7 @@ import sys
 
 REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 src, extra = sys.argv[1], sys.argv[2:]
-cmd = ["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-fno-gpu-rdc", "-ffp-contract=fast",
+cmd = ["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-fno-gpu-rdc", "-ffp-contract=fast", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
        "-I", os.path.join(REPO, "include"), *extra, "-Rpass-analysis=kernel-resource-usage", "-c",
        os.path.join(REPO, "cacophony_amd", "csrc", src), "-o", "/tmp/_regs.o"]
 out = subprocess.run(cmd, capture_output=True, text=True).stderr

@@ -25,7 +25,7 @@ def main():
     so = os.path.join(HERE, "probes", "libmfma_power.so")
     src = os.path.join(HERE, "probes", "mfma_power.hip")
     if not os.path.exists(so) or os.path.getmtime(so) < os.path.getmtime(src):
-        subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-shared", "-fPIC", src, "-o", so])
+        subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-shared", "-fPIC", src, "-o", so])
     lib = C.CDLL(so)
     lib.mfma_power_run.restype = C.c_double
     lib.mfma_power_run.argtypes = [C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]
