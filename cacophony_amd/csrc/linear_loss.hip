@@ -379,7 +379,7 @@ __global__ __launch_bounds__(256) void target_logits_kernel(LossArgs a) {
     const float q = a.tgt_q[first + entry];
     if (word >= 0 && g != 0.f && q != 0.f) {
       const unsigned x = max(float_exponent(g * q), 1u);      // below the normal numbers the units stay the same
-      if (a.dbe[word] < x) atomicMax(a.dbe + word, x);        // it only grows: an old value costs an atomic, not an answer
+      if (vg_peek(a.dbe + word) < x) atomicMax(a.dbe + word, x);      // it only grows: an old value costs an atomic, not an answer
     }
   }
 }

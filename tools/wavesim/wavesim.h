@@ -210,8 +210,8 @@ static inline void __builtin_amdgcn_sched_group_barrier(int, int, int) {}
 static inline void __builtin_amdgcn_sched_barrier(int) {}
 static inline void __builtin_amdgcn_s_setprio(int) {}
 // points where the lanes of a wave exchange data through LDS (common.h CACO_WAVE_LDS_SYNC, __builtin_amdgcn_wave_barrier)
-static inline __attribute__((noinline)) void wavesim_wave_sync() { wavesim::wave_rendezvous(__builtin_return_address(0)); }
-static inline __attribute__((noinline)) void __builtin_amdgcn_wave_barrier() { wavesim::wave_rendezvous(__builtin_return_address(0)); }
+static inline __attribute__((noinline, noduplicate)) void wavesim_wave_sync() { wavesim::wave_rendezvous(__builtin_return_address(0)); }
+static inline __attribute__((noinline, noduplicate)) void __builtin_amdgcn_wave_barrier() { wavesim::wave_rendezvous(__builtin_return_address(0)); }
 static inline void __builtin_amdgcn_s_barrier() { wavesim::block_barrier(); }
 static inline void __syncthreads() { wavesim::vm_wait(0); wavesim::block_barrier(); }
 static inline int __syncthreads_or(int pred) { wavesim::vm_wait(0); return wavesim::block_barrier_or(pred); }
@@ -235,21 +235,21 @@ static inline T wavesim_exchange_from(T v, int src_lane, const void* site) {
 }
 #define WAVESIM_SITE() __builtin_return_address(0)
 template <typename T>
-static inline __attribute__((noinline)) T __shfl_xor(T v, int mask, int width = 64) {
+static inline __attribute__((noinline, noduplicate)) T __shfl_xor(T v, int mask, int width = 64) {
   (void)width;
   return wavesim_exchange_from(v, wavesim::cur->lane ^ mask, WAVESIM_SITE());
 }
 template <typename T>
-static inline __attribute__((noinline)) T __shfl(T v, int src, int width = 64) {
+static inline __attribute__((noinline, noduplicate)) T __shfl(T v, int src, int width = 64) {
   const int base = wavesim::cur->lane & ~(width - 1);
   return wavesim_exchange_from(v, base + (src & (width - 1)), WAVESIM_SITE());
 }
 template <typename T>
-static inline __attribute__((noinline)) T __shfl_down(T v, unsigned d, int width = 64) {
+static inline __attribute__((noinline, noduplicate)) T __shfl_down(T v, unsigned d, int width = 64) {
   const int l = wavesim::cur->lane, s = l + (int)d;
   return wavesim_exchange_from(v, (s & ~(width - 1)) == (l & ~(width - 1)) ? s : l, WAVESIM_SITE());
 }
-static inline __attribute__((noinline)) unsigned long long __ballot(int pred) {
+static inline __attribute__((noinline, noduplicate)) unsigned long long __ballot(int pred) {
   *wavesim::xput() = pred ? 1 : 0;
   wavesim::wave_rendezvous(WAVESIM_SITE());
   unsigned long long m = 0;
@@ -258,7 +258,7 @@ static inline __attribute__((noinline)) unsigned long long __ballot(int pred) {
   return m;
 }
 template <typename T>
-static inline __attribute__((noinline)) T __builtin_amdgcn_readfirstlane(T v) {
+static inline __attribute__((noinline, noduplicate)) T __builtin_amdgcn_readfirstlane(T v) {
   memcpy(wavesim::xput(), &v, sizeof(T));
   wavesim::wave_rendezvous(WAVESIM_SITE());
   for (int l = 0; l < 64; ++l)
@@ -267,7 +267,7 @@ static inline __attribute__((noinline)) T __builtin_amdgcn_readfirstlane(T v) {
 }
 typedef unsigned int wavesim_u32x2 __attribute__((ext_vector_type(2)));
 // v_permlane32_swap vdst, src: lanes 32..63 of vdst trade places with lanes 0..31 of src; returns {vdst, src}
-static inline __attribute__((noinline)) wavesim_u32x2 __builtin_amdgcn_permlane32_swap(unsigned vdst, unsigned src, bool, bool) {
+static inline __attribute__((noinline, noduplicate)) wavesim_u32x2 __builtin_amdgcn_permlane32_swap(unsigned vdst, unsigned src, bool, bool) {
   unsigned both[2] = {vdst, src};
   memcpy(wavesim::xput(), both, 8);
   wavesim::wave_rendezvous(WAVESIM_SITE());
@@ -356,7 +356,7 @@ typedef __attribute__((address_space(3))) wavesim_s16x4* wavesim_lds_s16x4_ptr;
 // ds_read_b64_tr_b16: within each group of 16 lanes the 16 x 8-byte reads form a 4 x 16 matrix of 16-bit elements
 // distributed row-major (lane = row * 4 + col / 4, element = col % 4); it is returned column-major: lane n of the group
 // receives column n, i.e. element e of its result is element n % 4 of what lane e * 4 + n / 4 of the group read.
-static inline __attribute__((noinline)) wavesim_s16x4 __builtin_amdgcn_ds_read_tr16_b64_v4i16(wavesim_lds_s16x4_ptr p) {
+static inline __attribute__((noinline, noduplicate)) wavesim_s16x4 __builtin_amdgcn_ds_read_tr16_b64_v4i16(wavesim_lds_s16x4_ptr p) {
   memcpy(wavesim::xput(), reinterpret_cast<const void*>((uintptr_t)p), 8);
   wavesim::wave_rendezvous(WAVESIM_SITE());
   const int l = wavesim::cur->lane, g = l & ~15, n = l & 15;
@@ -378,7 +378,7 @@ typedef float wavesim_f32x16 __attribute__((ext_vector_type(16)));
 
 // v_mfma_f32_16x16x32_bf16: A[i][k] from lane i + 16 * (k / 8), element k % 8; B[k][j] likewise from lane j + 16 * (k / 8);
 // D[i][j]: lane j + 16 * (i / 4), register i % 4
-static inline __attribute__((noinline)) wavesim_f32x4 __builtin_amdgcn_mfma_f32_16x16x32_bf16(wavesim_bf16x8 a, wavesim_bf16x8 b, wavesim_f32x4 c,
+static inline __attribute__((noinline, noduplicate)) wavesim_f32x4 __builtin_amdgcn_mfma_f32_16x16x32_bf16(wavesim_bf16x8 a, wavesim_bf16x8 b, wavesim_f32x4 c,
                                                                                       int, int, int) {
   unsigned char* x = wavesim::xput();
   memcpy(x, &a, 16);
@@ -401,7 +401,7 @@ static inline __attribute__((noinline)) wavesim_f32x4 __builtin_amdgcn_mfma_f32_
 }
 // v_mfma_f32_32x32x16_bf16: A[i][k] from lane i + 32 * (k / 8), element k % 8; B likewise;
 // D[i][j]: lane j + 32 * ((i / 4) % 2), register (i / 8) * 4 + i % 4
-static inline __attribute__((noinline)) wavesim_f32x16 __builtin_amdgcn_mfma_f32_32x32x16_bf16(wavesim_bf16x8 a, wavesim_bf16x8 b, wavesim_f32x16 c,
+static inline __attribute__((noinline, noduplicate)) wavesim_f32x16 __builtin_amdgcn_mfma_f32_32x32x16_bf16(wavesim_bf16x8 a, wavesim_bf16x8 b, wavesim_f32x16 c,
                                                                                        int, int, int) {
   unsigned char* x = wavesim::xput();
   memcpy(x, &a, 16);
@@ -423,7 +423,7 @@ static inline __attribute__((noinline)) wavesim_f32x16 __builtin_amdgcn_mfma_f32
   return c;
 }
 // v_mfma_f32_32x32x2_f32: A[i][k] from lane i + 32 * k; B[k][j] from lane j + 32 * k; D as above.  Exact fp32 fma chain.
-static inline __attribute__((noinline)) wavesim_f32x16 __builtin_amdgcn_mfma_f32_32x32x2f32(float a, float b, wavesim_f32x16 c, int, int, int) {
+static inline __attribute__((noinline, noduplicate)) wavesim_f32x16 __builtin_amdgcn_mfma_f32_32x32x2f32(float a, float b, wavesim_f32x16 c, int, int, int) {
   unsigned char* x = wavesim::xput();
   memcpy(x, &a, 4);
   memcpy(x + 4, &b, 4);
