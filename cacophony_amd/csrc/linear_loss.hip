@@ -92,8 +92,8 @@ struct LossArgs {
   float* tgt_z;                      // distillation: the entries' logits [npad, kp]
   // compact: lse in log2 units is lse2 + a rest of at most 0.6 (see split_lse); the row's weight in the gradients g, and g 2^-rest
   float *lse2, *g, *gr;
-  // distillation, d bias: per word the exponent field of the largest |g q| of its entries, and their sum as an integer (see targets2_kernel)
-  unsigned* dbe; unsigned long long* db64;
+  // distillation, d bias: sums of g q per word as integers [16 ranges of exponents, vpad], and whether one is not finite (see targets2_kernel)
+  unsigned long long* db64; unsigned* dbn;
   // d logits of the piece in blocks of 256 rows x 256 columns, [row block][column block][256][256], once with the columns next to one another
   // (d hidden sums over them) and once with the rows (d weight): both products then read fragments of 16 bytes.  (One copy and
   // transposing reads in one of the products: 2.2 us per K-tile of it instead of 1.6; those reads and the loads into LDS get in each
@@ -176,9 +176,6 @@ __global__ __launch_bounds__(256) void targets_kernel(LossArgs a) {
 // the 256 x 256 block of d logits that holds (row, col)
 __device__ __forceinline__ int64_t dl_block(const LossArgs& a, int64_t row, int col) { return ((row >> 8) * (a.piece >> 8) + (col >> 8)) * 65536; }
 
-// the exponent field: 0 for zero and what lies below the normal numbers, 255 for NaN and the infinities
-__device__ __forceinline__ unsigned float_exponent(float x) { return __float_as_uint(x) >> 23 & 255; }
-
 // does row r count?
 __device__ __forceinline__ bool row_counts(const LossArgs& a, int64_t r) {
   if (a.labels) {
@@ -258,11 +255,12 @@ __global__ __launch_bounds__(256) void gather_kernel(LossArgs a, int backward, i
   }
   const int* rowmap = FEW ? s_row : a.rowmap;
   const int h0 = blockIdx.y * 64;
-  if (backward && a.db && a.topk)
-    for (int64_t v = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + t; v < a.vocab; v += (int64_t)gridDim.x * gridDim.y * 256) {
-      a.db64[v] = 0;
-      a.dbe[v] = 0;
-    }
+  if (backward && a.db && a.topk) {
+    const int64_t all = (int64_t)gridDim.x * gridDim.y * 256, at = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + t;
+    typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+    for (int64_t v = at; v < 8 * a.vpad; v += all) reinterpret_cast<u64x2*>(a.db64)[v] = u64x2{0, 0};
+    for (int64_t v = at; v < a.vpad; v += all) a.dbn[v] = 0;
+  }
   if (c0 >= ((int64_t)n + 255) / 256 * 256) return;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -338,49 +336,56 @@ __global__ __launch_bounds__(256) void transpose_kernel(const bf16_t* src, int64
 // (distillation) The entries' logits: a wave takes 16 entries of a compact row at a time, their rows of weight gathered.  The same instruction
 // as in the tiles, over k in the same order and from the same first sum, so that an entry has the bits its word's logit has in `lse` and `dlogits`:
 // what is left when it is taken from the row's reference has no rounding at the logits' size.  15 of the 16 columns of a product are
-// spent for that; what the kernel takes is the gathers' latency (16 rows x 64 bytes in one load, eight loads on their way).
-// With d bias, each entry also leaves its exponent with its word.
+// spent for that; what the kernel takes is the gathers' latency (eight loads of 8 rows x 128 bytes on their way) and, where the vocabulary is small
+// enough to stay in the L2s, their bandwidth: whole lines through the LDS there, since loads in the products' own layout, half a line of every
+// row, fetch the lines twice (2048 x 400 x 768, 128 entries: 58 us, with whole lines 27).
 constexpr int target_waves(int kp) { return kp > 32 ? 4 : kp > 16 ? 2 : 1; }      // waves of a row
 __global__ __launch_bounds__(256) void target_logits_kernel(LossArgs a) {
+  __shared__ bf16x8 s_w[4][4][128], s_h[4][32];      // a wave's 16 rows x 256 k in four K-tiles, chunk c of row r at c ^ (r & 7); its row's hidden states
   const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4, wave = threadIdx.x >> 6;
   const int waves = target_waves(a.kp), part = wave & (waves - 1);
   const int64_t c = (int64_t)blockIdx.x * (4 / waves) + wave / waves;
   if (c >= *a.count) return;
   const bf16_t* h = a.hc + c * a.hp;
-  const float g = a.db ? a.g[c] : 0.f;
   for (int e0 = part * 16; e0 < a.kp; e0 += 16 * waves) {
     const int64_t first = c * a.kp + e0;
     const int idx = e0 + l16 < a.kp ? a.tgt_idx[first + l16] : -1;      // of the row of weight that this lane brings
-    const bf16_t* w = a.weight + (int64_t)max(idx, 0) * a.ld_w;
     const float b = a.bias && idx >= 0 ? a.bias[idx] : 0.f;
     f32x4 acc;
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = __shfl(b, lq * 4 + e, 64);
+    const int r8 = lane >> 3, c8 = lane & 7;      // loading: rows r8 and r8 + 8, 16-byte chunk c8 of a line
+    const bf16_t* wr[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) wr[i] = a.weight + (int64_t)max(__shfl(idx, i * 8 + r8, 64), 0) * a.ld_w;      // an absent entry reads word 0, its logit is not used
     for (int k0 = 0; k0 < a.dim; k0 += 256) {
-      bf16x8 x[8], y[8];      // an absent entry reads word 0, its logit is not used
+      bf16x8 y[4][2], x = {};
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int k = k0 + u * 32 + lq * 8;
-        x[u] = *reinterpret_cast<const bf16x8*>(h + min(k, a.dim - 8));
-        y[u] = *reinterpret_cast<const bf16x8*>(w + min(k, a.dim - 8));
-      }
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        if (k0 + u * 32 + lq * 8 >= a.dim) x[u] = y[u] = bf16x8{};
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[u], x[u], acc, 0, 0, 0);
-      }
+        for (int i = 0; i < 2; ++i) y[t][i] = *reinterpret_cast<const bf16x8*>(wr[i] + min(k0 + t * 64 + c8 * 8, a.dim - 8));
+      if (lane < 32 && k0 + lane * 8 < a.dim) x = *reinterpret_cast<const bf16x8*>(h + k0 + lane * 8);
+      if (lane < 32) s_h[wave][lane] = x;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (k0 + t * 64 + c8 * 8 >= a.dim) y[t][i] = bf16x8{};
+          s_w[wave][t][(i * 8 + r8) * 8 + (c8 ^ r8)] = y[t][i];
+        }
+      CACO_WAVE_LDS_SYNC();
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(s_w[wave][t][l16 * 8 + ((u * 4 + lq) ^ (l16 & 7))], s_h[wave][t * 8 + u * 4 + lq], acc, 0, 0, 0);
+      CACO_WAVE_LDS_SYNC();
     }
     // every column holds the row's logits, those of entries lq * 4 .. + 3 in this lane: lanes l16 = 0 .. 3 take one each
     const int entry = lq * 4 + l16;
     if (l16 >= 4 || e0 + entry >= a.kp) continue;
     const float z = l16 == 0 ? acc[0] : l16 == 1 ? acc[1] : l16 == 2 ? acc[2] : acc[3];
     a.tgt_z[first + entry] = z;
-    const int word = a.tgt_idx[first + entry];
-    const float q = a.tgt_q[first + entry];
-    if (word >= 0 && g != 0.f && q != 0.f) {
-      const unsigned x = max(float_exponent(g * q), 1u);      // below the normal numbers the units stay the same
-      if (vg_peek(a.dbe + word) < x) atomicMax(a.dbe + word, x);      // it only grows: an old value costs an atomic, not an answer
-    }
   }
 }
 
@@ -855,9 +860,9 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
 }
 
 // (distillation) d logits at the teacher's tokens of the piece: one thread per entry.  The tokens of a row are distinct, so an entry is
-// written by one thread.  Their share of d bias, g q, is added as 64-bit integers, whose sum does not depend on the order.  A word has units of its
-// own: with E the exponent field of its largest |g q|, that one is below 2^(E - 126) = 2^39 units, the sum of 2^22 rows below 2^61, and what an
-// entry loses is at most 2^-39 of the largest, less than the roundings of a sum in fp32.  E = 255: one of them is not finite, and `dbias` says so.
+// written by one thread.  Their share of d bias, g q, is added up exactly, as integers, whose sum does not depend on the order: 16 sums for a word, one for every
+// 16 exponents, so that a share is its 24 bits shifted by 15 at most, and the sum of 2^22 rows stays below 2^61.  (One sum in units that the word's largest share
+// sets takes a pass of its own to find that one: 36 us where 2048 x 128 entries meet on 400 words.)  A share that is not finite marks the word.
 __global__ __launch_bounds__(256) void targets2_kernel(LossArgs a) {
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t c = t / a.kp;
@@ -870,8 +875,14 @@ __global__ __launch_bounds__(256) void targets2_kernel(LossArgs a) {
   a.dl[block + (c & 255) * 256 + (v & 255)] = d;
   if (a.dw) a.dlt[block + (v & 255) * 256 + (c & 255)] = d;
   if (!a.db) return;
-  const int E = (int)a.dbe[idx];
-  if (E < 255) atomicAdd(a.db64 + idx, (unsigned long long)(long long)rintf(ldexpf(g * q, 39 + 126 - E)));
+  const unsigned u = __float_as_uint(g * q);
+  const int E = u >> 23 & 255;
+  if (E == 255) {
+    atomicMax(a.dbn + idx, 1u);
+    return;
+  }
+  const long long m = (long long)((u & 0x7fffff) | (E ? 0x800000 : 0)) << (max(E, 1) - (E & ~15));      // in units of 2^((E & ~15) - 150)
+  atomicAdd(a.db64 + (int64_t)(E >> 4) * a.vpad + idx, (unsigned long long)(u >> 31 ? -m : m));
 }
 
 // How a piece's gradient work is shared out, XCD by XCD.
@@ -1053,7 +1064,12 @@ __device__ __forceinline__ void dbias(const LossArgs& a, int v, int bm, int wm) 
   float s = 0.f;
 #pragma unroll 8
   for (int p = 0; p < parts; ++p) s += a.dbp[p * a.vpad + v];
-  if (a.topk) s = a.dbe[v] < 255 ? (float)((double)s - ldexp((double)(long long)a.db64[v], (int)a.dbe[v] - 126 - 39)) : NAN;
+  if (a.topk) {
+    double t = 0., unit = 0x1p-150;
+#pragma unroll
+    for (int b = 0; b < 16; ++b, unit *= 0x1p16) t += (double)(long long)a.db64[b * a.vpad + v] * unit;
+    s = a.dbn[v] ? NAN : (float)((double)s - t);
+  }
   a.db[v] = s * common_scale(a, *a.count);
 }
 
@@ -1148,7 +1164,7 @@ struct Plan {
   int64_t piece;
   bool small;
   int lw = 0;
-  int64_t o_wslab = 0, o_count, o_sums, o_some, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_hct, o_part, o_zt, o_lse2, o_g, o_gr, o_db64, o_dbe, o_dl, o_dlt, o_wt, o_slab, o_dbp;
+  int64_t o_wslab = 0, o_count, o_sums, o_some, o_rowmap, o_inv, o_ti0, o_tq0, o_ti, o_tq, o_tz, o_hc, o_hct, o_part, o_zt, o_lse2, o_g, o_gr, o_db64, o_dbn, o_dl, o_dlt, o_wt, o_slab, o_dbp;
   int64_t take(int64_t n) {
     const int64_t at = bytes;
     bytes += up(n, 256);
@@ -1176,13 +1192,14 @@ struct Plan {
     o_part = take(most_groups(npad / bm) * (small ? MAX_WG : MAX_CU) * bm * 8);
     o_zt = take(npad * 4);
     piece = piece_cols;
-    o_lse2 = o_g = o_gr = o_hct = o_db64 = o_dbe = o_dl = o_dlt = o_slab = o_dbp = 0;
+    o_lse2 = o_g = o_gr = o_hct = o_db64 = o_dbn = o_dl = o_dlt = o_slab = o_dbp = 0;
     o_wt = -1;
     if (piece) {
       o_lse2 = take(npad * 4);
       o_g = take(npad * 4);
       o_gr = take(npad * 4);
-      if (topk) o_db64 = take((int64_t)vocab * 8), o_dbe = take((int64_t)vocab * 4);
+      vpad = up(vocab, 256);
+      if (topk) o_db64 = take(16 * vpad * 8), o_dbn = take(vpad * 4);
       o_hct = take((int64_t)hp * npad * 2);
       o_dl = take(npad * piece * 2);
       o_dlt = take(npad * piece * 2);
@@ -1194,7 +1211,6 @@ struct Plan {
       const int64_t wtiles = (int64_t)(vocab + 255) / 256 * ((dim + 255) / 256);
       while (npad >= 1536 && (wtiles << (lw + 1)) <= MAX_CU && (npad / VG_K >> (lw + 1)) >= 8) ++lw;
       if (lw) o_wslab = take((wtiles << lw) * 65536 * 4);
-      vpad = up(vocab, 256);
       o_dbp = take(npad / bm * (small ? Small::WM : Big::WM) * vpad * 4);
     }
   }
@@ -1329,7 +1345,7 @@ int linear_loss(const LinearLoss& c, hipStream_t st) {
   a.hc = (bf16_t*)(w + P.o_hc); a.hct = (bf16_t*)(w + P.o_hct); a.part = (float2*)(w + P.o_part); a.zt = (float*)(w + P.o_zt); a.tgt_z = (float*)(w + P.o_tz); 
   a.lse2 = (float*)(w + P.o_lse2); a.g = (float*)(w + P.o_g); a.gr = bwd ? (float*)(w + P.o_gr) : nullptr;
   a.dl = (bf16_t*)(w + P.o_dl); a.dlt = (bf16_t*)(w + P.o_dlt); a.wt = P.o_wt >= 0 && c.d_hidden ? (bf16_t*)(w + P.o_wt) : nullptr; a.slab = (float*)(w + P.o_slab); a.wslab = (float*)(w + P.o_wslab); a.lw = P.lw; a.dbp = (float*)(w + P.o_dbp); a.vpad = P.vpad;
-  a.arrived = (unsigned*)(a.count + 1); a.sums = (double*)(w + P.o_sums); a.db64 = (unsigned long long*)(w + P.o_db64); a.dbe = (unsigned*)(w + P.o_dbe);
+  a.arrived = (unsigned*)(a.count + 1); a.sums = (double*)(w + P.o_sums); a.db64 = (unsigned long long*)(w + P.o_db64); a.dbn = (unsigned*)(w + P.o_dbn);
   a.piece = (int)piece;
   int num_cu = 0;
   CACO_TRY_RC(prepare_launch(reinterpret_cast<const void*>(&lse_kernel<Big>), Big::SMEM_WFAR, &num_cu));
